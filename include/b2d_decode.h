@@ -54,7 +54,8 @@ enum b2d_status {
   B2D_ERR_CUDA = -5,             /* a CUDA runtime/driver call failed       */
   B2D_ERR_DEVICE_TIMEOUT = -6,   /* a kernel gave up waiting (status word)  */
   B2D_ERR_DEVICE_BOUNDS = -7,    /* a kernel saw a page id out of range     */
-  B2D_ERR_TOO_LARGE = -8         /* a size beyond the documented maximum    */
+  B2D_ERR_TOO_LARGE = -8,        /* a size beyond the documented maximum    */
+  B2D_ERR_DEVICE_CAPACITY = -9   /* pages, table or slots too few (status)  */
 };
 
 /* Launch flags, for measuring the two kernels of a decode separately.
@@ -241,6 +242,177 @@ typedef struct b2d_append_args {
 } b2d_append_args;
 
 int b2d_append_kv(const b2d_append_args* args, void* stream);
+
+/*
+ * Cross attention: ragged query tokens over paged states of another length
+ * (an encoder's, or any keys that every query token may see: no causal
+ * mask).  Query token t of request g reads all kv_lens[g] states of request
+ * g.  No counterpart in the reference.
+ *   q, out     [num_tokens, num_q_heads, head_dim] (bf16 | fp16)
+ *   caches     as those of b2d_decode_gqa, in any of its layouts
+ *   query_starts int32 [num_groups + 1]: request g owns tokens
+ *              [query_starts[g], query_starts[g + 1]), in ascending order.
+ *              NULL: query_len tokens each (num_tokens = num_groups * query_len)
+ *   kv_lens    int32 [num_groups], block_table int32 [num_groups,
+ *              max_pages_per_seq]
+ *   lse        [num_tokens, num_q_heads] fp32 (may be NULL)
+ * A request without states yields out = 0 and lse = -inf; tokens behind
+ * query_starts[num_groups] are left as they were.  head_dim 64, 128, 192 and
+ * 256, group (num_q_heads / num_kv_heads) <= 32.
+ */
+typedef struct b2d_cross_args {
+  const void* q;
+  int64_t q_stride_t, q_stride_h;
+  const void* k_cache;
+  const void* v_cache;
+  int64_t k_stride_page, k_stride_tok, k_stride_head;
+  int64_t v_stride_page, v_stride_tok, v_stride_head;
+  int64_t num_pages;
+  const int32_t* query_starts;
+  const int32_t* kv_lens;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const float* k_scale;
+  const float* v_scale;
+  void* out;
+  int64_t out_stride_t, out_stride_h;
+  float* lse;
+  int64_t lse_stride_t;
+  int32_t num_tokens, num_groups, query_len;
+  int32_t num_q_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq;
+  int32_t q_dtype, kv_dtype;
+  float softmax_scale;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t num_ctas;        /* 0 = one resident wave on this device          */
+  int32_t flags;           /* B2D_FLAG_TEST_NO_LOADS or 0                   */
+  int32_t kv_layout;       /* B2D_KV_*                                      */
+  int32_t wait_limit_us;   /* in-kernel wait limit, microseconds (0 = 2 s)  */
+} b2d_cross_args;
+
+/* Workspace bytes for these arguments (pointers may be NULL); the workspace
+ * starts with the same header as b2d_decode_gqa's. */
+int b2d_cross_workspace_bytes(const b2d_cross_args* args, size_t* bytes);
+int b2d_cross_attention(const b2d_cross_args* args, void* stream);
+
+/*
+ * Decode of a batch whose sequences share prefixes: sequence b attends to
+ * the prefix of its group, then to its own tokens.  The prefix is read once
+ * for all sequences of the group (as one matrix product per KV head) instead
+ * of once for each.  No counterpart in the reference.
+ *   own        the decode of the sequences' own tokens: cache_seqlens and
+ *              block_table describe these alone; out and lse are the result
+ *              over prefix and own tokens.  flags: 0 or TEST_NO_LOADS.
+ *   prefix_lens int32 [num_groups], prefix_block_table int32 [num_groups,
+ *              prefix_max_pages]: pages in the same caches
+ *   group_starts int32 [num_groups + 1]: group g holds sequences
+ *              [group_starts[g], group_starts[g + 1]); sequences outside
+ *              every group have no prefix.  NULL: one group with all.
+ * Either part may be empty; both: out = 0, lse = -inf.  num_groups <= 4096.
+ */
+typedef struct b2d_shared_prefix_args {
+  b2d_gqa_args own;
+  const int32_t* prefix_lens;
+  const int32_t* prefix_block_table;
+  int64_t prefix_block_table_stride;
+  const int32_t* group_starts;
+  int32_t num_groups, prefix_max_pages;
+} b2d_shared_prefix_args;
+
+int b2d_shared_prefix_workspace_bytes(const b2d_shared_prefix_args* args, size_t* bytes);
+int b2d_decode_shared_prefix(const b2d_shared_prefix_args* args, void* stream);
+
+/*
+ * Merge of attention states over disjoint parts of the keys (two caches, the
+ * ranks of a context-parallel decode): with M = max_i lse_i and w_i =
+ * e^(lse_i - M), out = sum w_i out_i / sum w_i, lse = M + ln sum w_i.  The
+ * rule of cute_attention/cluster_decode/cluster_decode_reduce.py:67-91 as a
+ * call of its own.  A state with lse = -inf is not read; rows in which all
+ * are: out = 0, lse = -inf.
+ *   outs [num_states, num_tokens, num_heads, head_dim] in in_dtype (bf16 |
+ *        fp16 | fp32), lses [num_states, num_tokens, num_heads] fp32
+ *   out  [num_tokens, num_heads, head_dim] in out_dtype (in_dtype, or bf16 |
+ *        fp16 from fp32), lse [num_tokens, num_heads] (may be NULL)
+ * head_dim: a multiple of 8 up to 1024.  out and lse overlap no input.
+ */
+typedef struct b2d_merge_args {
+  const void* outs;
+  int64_t outs_stride_n, outs_stride_t, outs_stride_h;
+  const float* lses;
+  int64_t lses_stride_n, lses_stride_t, lses_stride_h;
+  void* out;
+  int64_t out_stride_t, out_stride_h;
+  float* lse;
+  int64_t lse_stride_t, lse_stride_h;
+  int32_t num_states, num_tokens, num_heads, head_dim;
+  int32_t in_dtype, out_dtype;
+} b2d_merge_args;
+
+int b2d_merge_states(const b2d_merge_args* args, void* stream);
+
+/*
+ * Block tables and slot map of the next append, from request lengths: what a
+ * step needs between its scheduler and b2d_append_kv / b2d_decode_gqa.
+ * Request b holds cache_seqlens[b] tokens in ceil(cache_seqlens[b] /
+ * page_size) pages of its block_table row and gets new_tokens[b] more (NULL:
+ * one each).  Pages are taken from the top of the stack free_pages
+ * [0 .. *free_count): in request order, then page order, the k-th new page of
+ * the step is free_pages[*free_count - 1 - k].
+ *   block_table    [num_requests, max_pages_per_seq]: new pages written in place
+ *   slot_mapping   int64 [max_tokens]: slot of every new token, requests one
+ *                  after another; -1 behind the last (b2d_append_kv skips it)
+ *                  and where the table holds a negative page
+ *   query_starts   int32 [num_requests + 1]: first new token of each request
+ *   seqlens_out    int32 [num_requests], free_count_out int32 [1]: may be the
+ *                  input arrays (each step then continues the last)
+ * A step that does not fit changes nothing: when free pages, table columns or
+ * max_tokens are too few, block_table stays, seqlens_out = cache_seqlens,
+ * free_count_out = *free_count, all slots are -1, query_starts are 0, and the
+ * status word reports B2D_ERR_DEVICE_CAPACITY.  Negative lengths and counts
+ * count as 0.  num_requests <= 16384.  No counterpart in the reference.
+ */
+typedef struct b2d_plan_append_args {
+  const int32_t* cache_seqlens;
+  const int32_t* new_tokens;
+  int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int64_t* slot_mapping;
+  int32_t* query_starts;
+  int32_t* seqlens_out;
+  int32_t* free_count_out;
+  int32_t num_requests, max_pages_per_seq, page_size, max_tokens;
+  int32_t free_capacity;   /* entries of free_pages                         */
+  int32_t reserved;
+  void* workspace;         /* B2D_WORKSPACE_HEADER_BYTES, zero at first     */
+  size_t workspace_bytes;
+} b2d_plan_append_args;
+
+int b2d_plan_append(const b2d_plan_append_args* args, void* stream);
+
+/*
+ * The reverse: requests with finished[b] != 0 give all their pages back.  In
+ * request order, then page order, they are pushed onto free_pages behind
+ * *free_count; seqlens_out of such a request is 0.  block_table is only
+ * read.  When free_pages (free_capacity entries) has no room for all, nothing
+ * changes and the status word reports B2D_ERR_DEVICE_CAPACITY.
+ */
+typedef struct b2d_release_args {
+  const int32_t* cache_seqlens;
+  const uint8_t* finished;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* seqlens_out;
+  int32_t* free_count_out;
+  int32_t num_requests, max_pages_per_seq, page_size, free_capacity;
+  void* workspace;
+  size_t workspace_bytes;
+} b2d_release_args;
+
+int b2d_release_pages(const b2d_release_args* args, void* stream);
 
 /*
  * Reads (and clears, when clear != 0) the device status word that kernels

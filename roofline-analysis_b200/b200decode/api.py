@@ -49,7 +49,18 @@ class DecodeWorkspace:
     def __init__(self, device: torch.device, nbytes: int = 0, stream=None):
         self.device = torch.device(device)
         self.stream = stream
+        self.captured = False   # a CUDA graph holds this buffer's address
         self.buf = self._alloc(max(nbytes, 1 << 20))
+
+    @classmethod
+    def in_graph(cls, device: torch.device, nbytes: int) -> "DecodeWorkspace":
+        """A workspace of one call of a stream under capture: memory of the
+        graph's pool, its header zeroed by a node of the graph."""
+        ws = cls.__new__(cls)
+        ws.device, ws.stream, ws.captured = torch.device(device), None, True
+        ws.buf = torch.empty(max(nbytes, _lib.B2D_WORKSPACE_HEADER_BYTES), dtype=torch.uint8, device=device)
+        ws.buf[:_lib.B2D_WORKSPACE_HEADER_BYTES].zero_()
+        return ws
 
     def _alloc(self, n: int) -> torch.Tensor:
         if self.stream is None:
@@ -59,6 +70,9 @@ class DecodeWorkspace:
 
     def ensure(self, nbytes: int) -> "DecodeWorkspace":
         if self.buf.numel() < nbytes:
+            if self.captured:
+                raise ValueError(f"a workspace that a CUDA graph holds cannot grow (it has {self.buf.numel()} "
+                                 f"bytes, {nbytes} are needed): size it before the capture")
             self.buf = self._alloc(int(nbytes * 1.25) + 4096)
         return self
 

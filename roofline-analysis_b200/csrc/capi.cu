@@ -15,6 +15,8 @@ extern "C" const char* b2d_error_string(int status) {
     case B2D_ERR_DEVICE_TIMEOUT: return "a kernel gave up waiting on a pipeline barrier";
     case B2D_ERR_DEVICE_BOUNDS: return "a block-table page id was out of range";
     case B2D_ERR_TOO_LARGE: return "size beyond the supported maximum";
+    case B2D_ERR_DEVICE_CAPACITY:
+      return "a step found too few free pages, block-table columns or token slots";
     default: return "unknown b2d status";
   }
 }
@@ -37,6 +39,7 @@ extern "C" int b2d_check_device_status(void* workspace, int clear, void* stream)
   }
   if (word & 1) return B2D_ERR_DEVICE_TIMEOUT;
   if (word & 2) return B2D_ERR_DEVICE_BOUNDS;
+  if (word & 4) return B2D_ERR_DEVICE_CAPACITY;
   return B2D_OK;
 }
 

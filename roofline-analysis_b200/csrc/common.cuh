@@ -14,6 +14,7 @@ namespace b2d {
 // Status bits OR-ed into the workspace status word by kernels.
 constexpr int kStatusTimeout = 1;
 constexpr int kStatusBounds = 2;
+constexpr int kStatusCapacity = 4;
 
 // By default a wait on an mbarrier gives up after this many nanoseconds of
 // wall time (globaltimer).  No legitimate wait in these kernels comes near

@@ -421,7 +421,10 @@ extern "C" int b2d_gqa_plan(const b2d_gqa_args* a, int32_t* num_ctas, int32_t* c
   return B2D_OK;
 }
 
-static int decode_gqa(const b2d_gqa_args* a, void* stream, int* launch_count) {
+// out_f32: when set, out is written there in fp32 with the out strides of *a
+// (a->out is then not read or written).
+static int decode_gqa(const b2d_gqa_args* a, void* stream, int* launch_count,
+                      float* out_f32 = nullptr) {
   int rc = validate(a, launch_count == nullptr);
   if (rc) return rc;
   if (a->batch == 0) return B2D_OK;
@@ -450,6 +453,7 @@ static int decode_gqa(const b2d_gqa_args* a, void* stream, int* launch_count) {
     p.q_sb = a->q_stride_b;
     p.q_sh = a->q_stride_h;
     p.out = static_cast<uint8_t*>(a->out) + (size_t)b0 * a->out_stride_b * qes;
+    p.out_f32 = out_f32 ? out_f32 + (size_t)b0 * a->out_stride_b : nullptr;
     p.o_sb = a->out_stride_b;
     p.o_sh = a->out_stride_h;
     p.lse = a->lse ? a->lse + (size_t)b0 * a->lse_stride_b : nullptr;
@@ -494,6 +498,10 @@ static int decode_gqa(const b2d_gqa_args* a, void* stream, int* launch_count) {
 
 extern "C" int b2d_decode_gqa(const b2d_gqa_args* a, void* stream) {
   return decode_gqa(a, stream, nullptr);
+}
+
+int b2d::gqa_decode_f32(const b2d_gqa_args* a, float* out_f32, void* stream) {
+  return decode_gqa(a, stream, nullptr, out_f32);
 }
 
 extern "C" int b2d_gqa_launch_count(const b2d_gqa_args* a, int32_t* launches) {

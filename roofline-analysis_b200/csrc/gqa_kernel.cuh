@@ -49,6 +49,8 @@ struct GqaParams {
   const void* q;
   int64_t q_sb, q_sh;
   void* out;
+  float* out_f32;    // when set, out goes here in fp32 instead (same strides):
+                     // a part of a larger softmax, not yet rounded
   int64_t o_sb, o_sh;
   float* lse;
   int64_t lse_sb;
@@ -368,8 +370,14 @@ __global__ void __maxnreg__(B2D_GQA_MAXNREG)
       }
       if (cf == cl) {
         const int qh = hg * HQC + qh_row;
-        QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + c_in * 8;
-        store_out8<QT>(dst, o8);
+        const int64_t at = (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + c_in * 8;
+        if (p.out_f32 != nullptr) {
+          float4* dst = reinterpret_cast<float4*>(p.out_f32 + at);
+          dst[0] = make_float4(o8[0], o8[1], o8[2], o8[3]);
+          dst[1] = make_float4(o8[4], o8[5], o8[6], o8[7]);
+        } else {
+          store_out8<QT>(reinterpret_cast<QT*>(p.out) + at, o8);
+        }
         if (p.lse != nullptr && c_in == 0) p.lse[(int64_t)b * p.lse_sb + qh] = lse2 * kLn2;
       } else {
         const int64_t seg = (int64_t)row + cta;
@@ -599,10 +607,16 @@ __device__ __forceinline__ void warp_merge_heads(const GqaParams& p, int b, int 
     }
     if (live) {
       const int qh = hg * HQC + qh_row;
-      QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + hl * EPL;
+      const int64_t at = (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + hl * EPL;
       const float inv = 1.f / wsum;
+      if (p.out_f32 != nullptr) {
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) dst[e] = QT(acc[e] * inv);
+        for (int e = 0; e < EPL; ++e) p.out_f32[at + e] = acc[e] * inv;
+      } else {
+        QT* dst = reinterpret_cast<QT*>(p.out) + at;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) dst[e] = QT(acc[e] * inv);
+      }
       if (p.lse != nullptr && hl == 0) p.lse[(int64_t)b * p.lse_sb + qh] = (mx + fast_log2(wsum)) * kLn2;
     }
   }
@@ -617,9 +631,15 @@ __device__ __forceinline__ void warp_zero_heads(const GqaParams& p, int b, int h
   const int lane = threadIdx.x & 31;
   for (int hw = 0; hw < nh; ++hw) {
     const int qh = hg * HQC + qh_row0 + hw;
-    QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + lane * EPL;
+    const int64_t at = (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + lane * EPL;
+    if (p.out_f32 != nullptr) {
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) dst[e] = QT(0.f);
+      for (int e = 0; e < EPL; ++e) p.out_f32[at + e] = 0.f;
+    } else {
+      QT* dst = reinterpret_cast<QT*>(p.out) + at;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) dst[e] = QT(0.f);
+    }
     if (p.lse != nullptr && lane == 0) p.lse[(int64_t)b * p.lse_sb + qh] = -INFINITY;
   }
 }
@@ -667,10 +687,14 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(const GqaParams p, int
       }
     }
   }
-  QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + lane * EPL;
+  const int64_t at = (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + lane * EPL;
+  auto put = [&](int e, float v) {
+    if (p.out_f32 != nullptr) p.out_f32[at + e] = v;
+    else reinterpret_cast<QT*>(p.out)[at + e] = QT(v);
+  };
   if (mode == 1 && sub == 0) {
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) dst[e] = QT(0.f);
+    for (int e = 0; e < EPL; ++e) put(e, 0.f);
     if (p.lse != nullptr && lane == 0) p.lse[(int64_t)b * p.lse_sb + qh] = -INFINITY;
   }
   float acc[EPL];
@@ -720,7 +744,7 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(const GqaParams p, int
   if (mode == 2 && sub == 0) {
     const float inv = 1.f / wsum;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) dst[e] = QT(acc[e] * inv);
+    for (int e = 0; e < EPL; ++e) put(e, acc[e] * inv);
     if (p.lse != nullptr && lane == 0) p.lse[(int64_t)b * p.lse_sb + qh] = (mx + fast_log2(wsum)) * kLn2;
   }
 }

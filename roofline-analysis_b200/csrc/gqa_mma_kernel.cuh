@@ -337,12 +337,21 @@ __global__ void __launch_bounds__(32 * 9, 1)
         const float inv = vscale / lh;
         const int qh_row = qh_row0 + hw;
         if (cf == cl) {
-          QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t)b * p.o_sb +
-                    (int64_t)(hg * HQC + qh_row) * p.o_sh;
+          const int64_t at = (int64_t)b * p.o_sb + (int64_t)(hg * HQC + qh_row) * p.o_sh;
+          if (p.out_f32 != nullptr) {
+            float* dst = p.out_f32 + at;
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            dst[out_dim(i, 0)] = QT(acc[n][i][c] * inv);
-            dst[out_dim(i, 1)] = QT(acc[n][i][2 + c] * inv);
+            for (int i = 0; i < MT; ++i) {
+              dst[out_dim(i, 0)] = acc[n][i][c] * inv;
+              dst[out_dim(i, 1)] = acc[n][i][2 + c] * inv;
+            }
+          } else {
+            QT* dst = reinterpret_cast<QT*>(p.out) + at;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              dst[out_dim(i, 0)] = QT(acc[n][i][c] * inv);
+              dst[out_dim(i, 1)] = QT(acc[n][i][2 + c] * inv);
+            }
           }
           if (p.lse != nullptr && g == 0)
             p.lse[(int64_t)b * p.lse_sb + hg * HQC + qh_row] = (mh + fast_log2(lh)) * kLn2;

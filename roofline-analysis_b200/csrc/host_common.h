@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "b2d_decode.h"
+
 namespace b2d {
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
@@ -34,5 +36,9 @@ int encode_tiled_map(CUtensorMap* map, CUtensorMapDataType dtype, int rank, cons
 inline int combine_warps_per_merge(int64_t merges) {
   return merges <= 256 ? 8 : merges <= 512 ? 4 : merges <= 1024 ? 2 : 1;
 }
+
+// b2d_decode_gqa with out in fp32 (at out_f32, with the out strides of *args,
+// in elements): one part of a softmax that a later merge completes.
+int gqa_decode_f32(const ::b2d_gqa_args* args, float* out_f32, void* stream);
 
 }  // namespace b2d

@@ -1,0 +1,308 @@
+// pages.cu — block tables and slot maps from request lengths, and the return
+// of finished requests' pages: the integer work between a scheduler and the
+// append / decode calls, without a trip to the host.
+//
+// Math (P = page size, L = length, n = new tokens of a request):
+//   have = ceil(L / P), need = ceil((L + n) / P) - have
+//   token_start = exclusive sum of n, page_start = exclusive sum of need
+//   new page k of the step = free_pages[free_count - 1 - k]
+//   slot of token i of a request = page((L + i) / P) * P + (L + i) % P
+//
+// Bound by latency: a decode step moves a few KB, so the whole step is one
+// launch.  Every block computes the sums of all requests itself (a few KB
+// from L2, the sums stay in shared memory) and then does its share of the
+// slots and table entries, finding each one's request by bisection; no block
+// waits for another.  The lengths and the free count may be updated in
+// place: the block that is last to finish reading (an arrival counter in the
+// workspace header, zero between calls) writes them.
+#include "b2d_decode.h"
+#include "common.cuh"
+#include "host_common.h"
+
+namespace b2d {
+
+constexpr int kPageThreads = 512;
+constexpr int kMaxRequests = 16384;
+
+struct PagesParams {
+  const int32_t* lens;
+  const int32_t* new_tokens;    // append; null: one each
+  const uint8_t* finished;      // release
+  int32_t* table;
+  int64_t table_stride;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int64_t* slots;
+  int32_t* starts;
+  int32_t* lens_out;
+  int32_t* count_out;
+  int* status;
+  int* arrivals;
+  int B, max_pages, P, max_tokens, capacity;
+};
+
+__device__ __forceinline__ int64_t pages_of(int64_t tokens, int P) { return (tokens + P - 1) / P; }
+
+__device__ __forceinline__ int length_of(const PagesParams& p, int b) {
+  const int n = p.lens[b];
+  return n < 0 ? 0 : n;
+}
+
+__device__ __forceinline__ int new_of(const PagesParams& p, int b) {
+  if (p.new_tokens == nullptr) return 1;
+  const int n = p.new_tokens[b];
+  return n < 0 ? 0 : n;
+}
+
+// Exclusive block-wide sum of two 64-bit values per thread, and their totals.
+__device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t& ta, int64_t& tb) {
+  __shared__ int64_t wa[32], wb[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int64_t x = a, y = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) {
+      x += u;
+      y += v;
+    }
+  }
+  if (lane == 31) {
+    wa[warp] = x;
+    wb[warp] = y;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int64_t s = lane < nw ? wa[lane] : 0, t = lane < nw ? wb[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, s, o), v = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) {
+        s += u;
+        t += v;
+      }
+    }
+    wa[lane] = s;
+    wb[lane] = t;
+  }
+  __syncthreads();
+  a = x - a + (warp > 0 ? wa[warp - 1] : 0);
+  b = y - b + (warp > 0 ? wb[warp - 1] : 0);
+  ta = wa[nw - 1];
+  tb = wb[nw - 1];
+}
+
+// Last b with start[b] <= i (requests that got nothing come before it).
+__device__ __forceinline__ int request_of(const int32_t* start, int B, int i) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (start[mid] <= i) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// True in the block that arrives last: every other block has read its inputs.
+__device__ __forceinline__ bool last_block(int* arrivals) {
+  __shared__ int last;
+  __syncthreads();
+  if (gridDim.x == 1) return true;
+  if (threadIdx.x == 0) {
+    last = atomic_add_acq_rel_gpu(arrivals, 1) == (int)gridDim.x - 1;
+    if (last) *arrivals = 0;
+  }
+  __syncthreads();
+  return last != 0;
+}
+
+__global__ void __launch_bounds__(kPageThreads) plan_append_kernel(const PagesParams p) {
+  extern __shared__ int32_t sm[];
+  int32_t* tok_start = sm;          // [B]
+  int32_t* page_start = sm + p.B;   // [B]
+  const int tid = threadIdx.x;
+  const int per = (p.B + kPageThreads - 1) / kPageThreads;
+  const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  int64_t toks = 0, pages = 0;
+  bool fits = true;
+  for (int b = b0; b < b1; ++b) {
+    const int64_t L = length_of(p, b), n = new_of(p, b);
+    const int64_t end = pages_of(L + n, p.P);
+    toks += n;
+    pages += end - pages_of(L, p.P);
+    fits = fits && (n == 0 || end <= p.max_pages);
+  }
+  int64_t total_toks, total_pages;
+  block_scan2(toks, pages, total_toks, total_pages);
+  const int count_in = *p.free_count;
+  const int count = max(0, min(count_in, p.capacity));
+  fits = __syncthreads_and(fits && total_toks <= p.max_tokens && total_pages <= count);
+  for (int b = b0; b < b1; ++b) {   // used only when the totals fit 32 bits
+    tok_start[b] = (int)toks;
+    page_start[b] = (int)pages;
+    const int64_t L = length_of(p, b), n = new_of(p, b);
+    toks += n;
+    pages += pages_of(L + n, p.P) - pages_of(L, p.P);
+  }
+  __syncthreads();
+  const int first = blockIdx.x * kPageThreads + tid, step = gridDim.x * kPageThreads;
+  for (int b = first; b <= p.B; b += step)
+    p.starts[b] = !fits ? 0 : (b == p.B ? (int)total_toks : tok_start[b]);
+  const int nt = fits ? (int)total_toks : 0, np = fits ? (int)total_pages : 0;
+  for (int t = first; t < p.max_tokens; t += step) {
+    int64_t slot = -1;
+    if (t < nt) {
+      const int b = request_of(tok_start, p.B, t);
+      const int L = length_of(p, b), have = (int)pages_of(L, p.P);
+      const int pos = L + (t - tok_start[b]), pi = pos / p.P;
+      const int page = pi < have ? p.table[b * p.table_stride + pi]
+                                 : p.free_pages[count - 1 - (page_start[b] + pi - have)];
+      if (page >= 0) slot = (int64_t)page * p.P + (pos - pi * p.P);
+    }
+    p.slots[t] = slot;
+  }
+  for (int k = first; k < np; k += step) {
+    const int b = request_of(page_start, p.B, k);
+    const int have = (int)pages_of(length_of(p, b), p.P);
+    p.table[b * p.table_stride + have + (k - page_start[b])] = p.free_pages[count - 1 - k];
+  }
+  if (!last_block(p.arrivals)) return;
+  for (int b = tid; b < p.B; b += kPageThreads) {
+    const int n = new_of(p, b);
+    const int L = p.lens[b];
+    p.lens_out[b] = fits ? (L < 0 ? 0 : L) + n : L;
+  }
+  if (tid == 0) {
+    *p.count_out = fits ? count - np : count_in;
+    if (!fits) record_status(p.status, kStatusCapacity);
+  }
+}
+
+__global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const PagesParams p) {
+  extern __shared__ int32_t sm[];
+  int32_t* page_start = sm;   // [B]
+  const int tid = threadIdx.x;
+  const int per = (p.B + kPageThreads - 1) / kPageThreads;
+  const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  auto given = [&](int b) -> int64_t {
+    if (p.finished[b] == 0) return 0;
+    const int64_t n = pages_of(length_of(p, b), p.P);
+    return n < p.max_pages ? n : p.max_pages;
+  };
+  int64_t pages = 0, unused = 0, total, unused_total;
+  for (int b = b0; b < b1; ++b) pages += given(b);
+  block_scan2(pages, unused, total, unused_total);
+  const int count_in = *p.free_count;
+  const int count = max(0, min(count_in, p.capacity));
+  const bool fits = total <= p.capacity - count;
+  for (int b = b0; b < b1; ++b) {   // used only when the total fits 32 bits
+    page_start[b] = (int)pages;
+    pages += given(b);
+  }
+  __syncthreads();
+  const int np = fits ? (int)total : 0;
+  for (int k = blockIdx.x * kPageThreads + tid; k < np; k += gridDim.x * kPageThreads) {
+    const int b = request_of(page_start, p.B, k);
+    p.free_pages[count + k] = p.table[b * p.table_stride + (k - page_start[b])];
+  }
+  if (!last_block(p.arrivals)) return;
+  for (int b = tid; b < p.B; b += kPageThreads) {
+    const int L = p.lens[b];
+    p.lens_out[b] = fits && p.finished[b] ? 0 : L;
+  }
+  if (tid == 0) {
+    *p.count_out = fits ? count + np : count_in;
+    if (!fits) record_status(p.status, kStatusCapacity);
+  }
+}
+
+// Blocks for `work` entries: one per 2048, at most one per SM.
+static int page_blocks(int64_t work, int sms) {
+  const int64_t n = (work + 2047) / 2048;
+  return (int)(n < 1 ? 1 : (n > sms ? sms : n));
+}
+
+static int check_header(const void* ws, size_t bytes) {
+  if (!ws || bytes < kWsHeaderBytes) return B2D_ERR_WORKSPACE;
+  return ((uintptr_t)ws & 255) ? B2D_ERR_ALIGNMENT : B2D_OK;
+}
+
+}  // namespace b2d
+
+using namespace b2d;
+
+extern "C" int b2d_plan_append(const b2d_plan_append_args* a, void* stream) {
+  if (!a || a->num_requests < 0 || a->max_pages_per_seq <= 0 || a->page_size <= 0 ||
+      a->max_tokens < 0 || a->free_capacity < 0)
+    return B2D_ERR_INVALID_ARG;
+  if (a->num_requests > kMaxRequests ||
+      (int64_t)a->max_pages_per_seq * a->page_size > (int64_t)INT32_MAX)
+    return B2D_ERR_TOO_LARGE;
+  if ((a->num_requests > 0 && (!a->cache_seqlens || !a->block_table || !a->seqlens_out)) ||
+      !a->free_count || !a->free_count_out || !a->query_starts ||
+      (a->max_tokens > 0 && !a->slot_mapping) || (a->free_capacity > 0 && !a->free_pages))
+    return B2D_ERR_INVALID_ARG;
+  if (int rc = check_header(a->workspace, a->workspace_bytes)) return rc;
+  PagesParams p{};
+  p.lens = a->cache_seqlens;
+  p.new_tokens = a->new_tokens;
+  p.table = a->block_table;
+  p.table_stride = a->block_table_stride;
+  p.free_pages = const_cast<int32_t*>(a->free_pages);
+  p.free_count = a->free_count;
+  p.slots = a->slot_mapping;
+  p.starts = a->query_starts;
+  p.lens_out = a->seqlens_out;
+  p.count_out = a->free_count_out;
+  p.status = static_cast<int*>(a->workspace);
+  p.arrivals = reinterpret_cast<int*>(static_cast<uint8_t*>(a->workspace) + kStatusBytes);
+  p.B = a->num_requests;
+  p.max_pages = a->max_pages_per_seq;
+  p.P = a->page_size;
+  p.max_tokens = a->max_tokens;
+  p.capacity = a->free_capacity;
+  int sms = 0;
+  if (device_sm_count(&sms)) return B2D_ERR_CUDA;
+  const size_t smem = (size_t)p.B * 8;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(plan_append_kernel), smem)) return B2D_ERR_CUDA;
+  plan_append_kernel<<<page_blocks(p.max_tokens, sms), kPageThreads, smem,
+                       static_cast<cudaStream_t>(stream)>>>(p);
+  return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+}
+
+extern "C" int b2d_release_pages(const b2d_release_args* a, void* stream) {
+  if (!a || a->num_requests < 0 || a->max_pages_per_seq <= 0 || a->page_size <= 0 ||
+      a->free_capacity < 0)
+    return B2D_ERR_INVALID_ARG;
+  if (a->num_requests > kMaxRequests ||
+      (int64_t)a->max_pages_per_seq * a->page_size > (int64_t)INT32_MAX)
+    return B2D_ERR_TOO_LARGE;
+  if ((a->num_requests > 0 && (!a->cache_seqlens || !a->block_table || !a->finished ||
+                               !a->seqlens_out)) ||
+      !a->free_count || !a->free_count_out || (a->free_capacity > 0 && !a->free_pages))
+    return B2D_ERR_INVALID_ARG;
+  if (int rc = check_header(a->workspace, a->workspace_bytes)) return rc;
+  PagesParams p{};
+  p.lens = a->cache_seqlens;
+  p.finished = a->finished;
+  p.table = const_cast<int32_t*>(a->block_table);
+  p.table_stride = a->block_table_stride;
+  p.free_pages = a->free_pages;
+  p.free_count = a->free_count;
+  p.lens_out = a->seqlens_out;
+  p.count_out = a->free_count_out;
+  p.status = static_cast<int*>(a->workspace);
+  p.arrivals = reinterpret_cast<int*>(static_cast<uint8_t*>(a->workspace) + kStatusBytes);
+  p.B = a->num_requests;
+  p.max_pages = a->max_pages_per_seq;
+  p.P = a->page_size;
+  p.capacity = a->free_capacity;
+  int sms = 0;
+  if (device_sm_count(&sms)) return B2D_ERR_CUDA;
+  const size_t smem = (size_t)p.B * 4;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(release_pages_kernel), smem)) return B2D_ERR_CUDA;
+  // At most min(all requests' table columns, free capacity) pages come back.
+  const int64_t most = (int64_t)p.B * p.max_pages;
+  release_pages_kernel<<<page_blocks(most < p.capacity ? most : p.capacity, sms), kPageThreads, smem,
+                         static_cast<cudaStream_t>(stream)>>>(p);
+  return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+}

@@ -1,0 +1,355 @@
+// ragged_host.cu — host side of cross attention and shared-prefix decode:
+// argument checks, the choice of kernel, workspace layout and launches.
+#include <algorithm>
+
+#include "b2d_decode.h"
+#include "host_common.h"
+#include "ragged.cuh"
+#include "ragged_mma_kernel.cuh"
+
+namespace b2d {
+
+// Groups per launch: the chunk table of all of them sits in shared memory
+// (16 KB).  Cross attention runs longer lists in slices.
+constexpr int kMaxGroups = 4096;
+
+struct RaggedPlan {
+  int TS, CH, rows, threads, ctas;
+  size_t smem;
+  size_t off_table, off_seg_lse, off_seg_o, bytes;  // offsets from the plan's part of the workspace
+};
+
+static int check_sizes(const b2d_cross_args* a) {
+  if (a == nullptr) return B2D_ERR_INVALID_ARG;
+  if (a->num_tokens < 0 || a->num_groups < 0 || a->query_len < 0 || a->num_q_heads <= 0 ||
+      a->num_kv_heads <= 0 || a->page_size <= 0 || a->max_pages_per_seq <= 0)
+    return B2D_ERR_INVALID_ARG;
+  if (a->num_q_heads % a->num_kv_heads != 0) return B2D_ERR_INVALID_ARG;
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 192 && a->head_dim != 256)
+    return B2D_ERR_UNSUPPORTED;
+  if (a->q_dtype != B2D_BF16 && a->q_dtype != B2D_FP16) return B2D_ERR_UNSUPPORTED;
+  if (a->kv_dtype != a->q_dtype && a->kv_dtype != B2D_FP8_E4M3) return B2D_ERR_UNSUPPORTED;
+  if (a->num_q_heads / a->num_kv_heads > 32) return B2D_ERR_UNSUPPORTED;
+  if (a->page_size > (1 << 24)) return B2D_ERR_TOO_LARGE;
+  if ((int64_t)a->max_pages_per_seq * a->page_size > (int64_t)INT32_MAX) return B2D_ERR_TOO_LARGE;
+  if (a->wait_limit_us < 0) return B2D_ERR_INVALID_ARG;
+  if (a->kv_layout != B2D_KV_STRIDED && a->kv_layout != B2D_KV_VLLM) return B2D_ERR_INVALID_ARG;
+  if (a->kv_layout == B2D_KV_VLLM && (a->kv_dtype == B2D_FP8_E4M3 || a->page_size % 16 != 0))
+    return B2D_ERR_UNSUPPORTED;
+  return B2D_OK;
+}
+
+static int check_pointers(const b2d_cross_args* a) {
+  if (!a->q || !a->k_cache || !a->v_cache || !a->kv_lens || !a->block_table || !a->out)
+    return B2D_ERR_INVALID_ARG;
+  if (a->num_pages <= 0 || a->num_pages > (int64_t)INT32_MAX) return B2D_ERR_INVALID_ARG;
+  if (!a->query_starts && (int64_t)a->num_groups * a->query_len != a->num_tokens)
+    return B2D_ERR_INVALID_ARG;
+  const int es = a->kv_dtype == B2D_FP8_E4M3 ? 1 : 2;
+  if (((uintptr_t)a->k_cache & 15) || ((uintptr_t)a->v_cache & 15) || ((uintptr_t)a->q & 15) ||
+      ((uintptr_t)a->out & 15))
+    return B2D_ERR_ALIGNMENT;
+  const int64_t strides[6] = {a->k_stride_page, a->k_stride_tok, a->k_stride_head,
+                              a->v_stride_page, a->v_stride_tok, a->v_stride_head};
+  for (int i = 0; i < 6; ++i) {
+    if (a->kv_layout == B2D_KV_VLLM && (i == 1 || i == 4)) continue;  // token strides implied
+    if (strides[i] <= 0 || (strides[i] * es) % 16 != 0) return B2D_ERR_ALIGNMENT;
+  }
+  if ((a->q_stride_t * 2) % 16 || (a->q_stride_h * 2) % 16 || (a->out_stride_t * 2) % 16 ||
+      (a->out_stride_h * 2) % 16)
+    return B2D_ERR_ALIGNMENT;
+  return B2D_OK;
+}
+
+static int make_plan(const b2d_cross_args* a, RaggedPlan* pl) {
+  const int grp = a->num_q_heads / a->num_kv_heads;
+  const int groups = std::min(a->num_groups, kMaxGroups);
+  pl->rows = 64;
+  pl->threads = 128;
+  pl->CH = a->head_dim <= 128 ? 64 : 32;
+  pl->TS = pl->rows / grp;
+  pl->smem = (size_t)(pl->rows + 2 * pl->CH) * (a->head_dim + 8) * 2 + (size_t)(groups + 1) * 4 + 128;
+  pl->ctas = a->num_ctas;
+  if (pl->ctas <= 0) {
+    int sms = 0;
+    if (device_sm_count(&sms) != 0) return B2D_ERR_CUDA;
+    pl->ctas = 2 * sms;
+  }
+  // Positions on the chunk line are 32-bit in the kernels.
+  const int64_t chunks = ((int64_t)a->max_pages_per_seq * a->page_size + pl->CH - 1) / pl->CH;
+  const int64_t tiles = (int64_t)a->num_tokens / pl->TS + groups;
+  if (tiles * a->num_kv_heads > (int64_t)INT32_MAX / chunks) return B2D_ERR_TOO_LARGE;
+  const size_t seg_rows = (size_t)2 * pl->ctas * pl->rows;
+  pl->off_table = 0;
+  pl->off_seg_lse = align_up((size_t)(groups + 1) * 4, 256);
+  pl->off_seg_o = align_up(pl->off_seg_lse + seg_rows * 4, 256);
+  pl->bytes = align_up(pl->off_seg_o + seg_rows * a->head_dim * 4, 256);
+  return B2D_OK;
+}
+
+static RaggedParams params_of(const b2d_cross_args* a, const RaggedPlan& pl, uint8_t* part) {
+  RaggedParams p{};
+  p.q = a->q;
+  p.q_st = a->q_stride_t;
+  p.q_sh = a->q_stride_h;
+  p.kc = a->k_cache;
+  p.vc = a->v_cache;
+  p.k_sp = a->k_stride_page;
+  p.k_st = a->k_stride_tok;
+  p.k_sh = a->k_stride_head;
+  p.v_sp = a->v_stride_page;
+  p.v_st = a->v_stride_tok;
+  p.v_sh = a->v_stride_head;
+  p.k_sg = 8;
+  p.v_sd = 1;
+  if (a->kv_layout == B2D_KV_VLLM) {  // K [blocks, Hkv, D/8, P, 8], V [blocks, Hkv, D, P]
+    p.k_st = 8;
+    p.k_sg = (int64_t)a->page_size * 8;
+    p.v_st = 1;
+    p.v_sd = a->page_size;
+  }
+  p.starts = a->query_starts;
+  p.kv_lens = a->kv_lens;
+  p.block_table = a->block_table;
+  p.bt_stride = a->block_table_stride;
+  p.k_scale = a->k_scale;
+  p.v_scale = a->v_scale;
+  p.out = a->out;
+  p.o_st = a->out_stride_t;
+  p.o_sh = a->out_stride_h;
+  p.lse = a->lse;
+  p.lse_st = a->lse_stride_t;
+  p.table_g = reinterpret_cast<int32_t*>(part + pl.off_table);
+  p.seg_lse = reinterpret_cast<float*>(part + pl.off_seg_lse);
+  p.seg_o = reinterpret_cast<float*>(part + pl.off_seg_o);
+  p.status = static_cast<int*>(a->workspace);
+  p.wait_ns = a->wait_limit_us > 0 ? (unsigned long long)a->wait_limit_us * 1000ull : kWaitLimitNs;
+  p.no_loads = (a->flags & B2D_FLAG_TEST_NO_LOADS) ? 1 : 0;
+  p.G = a->num_groups;
+  p.T = a->num_tokens;
+  p.uniform = a->query_len;
+  p.Hq = a->num_q_heads;
+  p.Hkv = a->num_kv_heads;
+  p.grp = a->num_q_heads / a->num_kv_heads;
+  p.P = a->page_size;
+  p.num_pages = (int)a->num_pages;
+  p.max_pages = a->max_pages_per_seq;
+  p.TS = pl.TS;
+  p.CH = pl.CH;
+  p.rows = pl.rows;
+  p.scale = a->softmax_scale * 1.4426950408889634f;
+  return p;
+}
+
+template <int D, int KIND, typename QT>
+static int launch_mma(const RaggedPlan& pl, const RaggedParams& p, cudaStream_t st) {
+  auto kern = ragged_mma_kernel<D, KIND, QT>;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), pl.smem)) return B2D_ERR_CUDA;
+  kern<<<pl.ctas, pl.threads, pl.smem, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+}
+
+template <int D>
+static int launch_attention(const b2d_cross_args* a, const RaggedPlan& pl, const RaggedParams& p,
+                            cudaStream_t st) {
+  const bool bf = a->q_dtype == B2D_BF16;
+  if (a->kv_dtype == B2D_FP8_E4M3)
+    return bf ? launch_mma<D, kKvFp8, __nv_bfloat16>(pl, p, st)
+              : launch_mma<D, kKvFp8, __half>(pl, p, st);
+  return bf ? launch_mma<D, kKvBf16, __nv_bfloat16>(pl, p, st)
+            : launch_mma<D, kKvFp16, __half>(pl, p, st);
+}
+
+static int launch_attention(const b2d_cross_args* a, const RaggedPlan& pl, const RaggedParams& p,
+                            cudaStream_t st) {
+  switch (a->head_dim) {
+    case 64: return launch_attention<64>(a, pl, p, st);
+    case 128: return launch_attention<128>(a, pl, p, st);
+    case 192: return launch_attention<192>(a, pl, p, st);
+    default: return launch_attention<256>(a, pl, p, st);
+  }
+}
+
+template <int D, typename QT>
+static void launch_merge(const RaggedPlan& pl, const RaggedParams& p, cudaStream_t st) {
+  if (pl.ctas > 1)
+    ragged_merge_kernel<D, QT><<<dim3(pl.ctas - 1, pl.rows / 8), 256, 0, st>>>(p, pl.ctas);
+}
+
+template <int D, typename QT>
+static void launch_join(const RaggedPlan& pl, const RaggedParams& p, const float* own_o,
+                        const float* own_lse, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.T * p.Hq;
+  shared_join_kernel<D, QT><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, pl.ctas, own_o, own_lse);
+}
+
+#define B2D_BY_DIM_AND_TYPE(fn, dim, bf, ...)                                      \
+  do {                                                                             \
+    switch (dim) {                                                                 \
+      case 64: (bf) ? fn<64, __nv_bfloat16>(__VA_ARGS__) : fn<64, __half>(__VA_ARGS__); break;    \
+      case 128: (bf) ? fn<128, __nv_bfloat16>(__VA_ARGS__) : fn<128, __half>(__VA_ARGS__); break; \
+      case 192: (bf) ? fn<192, __nv_bfloat16>(__VA_ARGS__) : fn<192, __half>(__VA_ARGS__); break; \
+      default: (bf) ? fn<256, __nv_bfloat16>(__VA_ARGS__) : fn<256, __half>(__VA_ARGS__); break;  \
+    }                                                                              \
+  } while (0)
+
+// The prefix half of a shared-prefix decode as a ragged problem: the
+// sequences of a group are the tokens that read its prefix.
+static b2d_cross_args prefix_of(const b2d_shared_prefix_args* a) {
+  const b2d_gqa_args& o = a->own;
+  b2d_cross_args c{};
+  c.q = o.q;
+  c.q_stride_t = o.q_stride_b;
+  c.q_stride_h = o.q_stride_h;
+  c.k_cache = o.k_cache;
+  c.v_cache = o.v_cache;
+  c.k_stride_page = o.k_stride_page;
+  c.k_stride_tok = o.k_stride_tok;
+  c.k_stride_head = o.k_stride_head;
+  c.v_stride_page = o.v_stride_page;
+  c.v_stride_tok = o.v_stride_tok;
+  c.v_stride_head = o.v_stride_head;
+  c.num_pages = o.num_pages;
+  c.query_starts = a->group_starts;
+  c.kv_lens = a->prefix_lens;
+  c.block_table = a->prefix_block_table;
+  c.block_table_stride = a->prefix_block_table_stride;
+  c.k_scale = o.k_scale;
+  c.v_scale = o.v_scale;
+  c.out = o.out;
+  c.out_stride_t = o.out_stride_b;
+  c.out_stride_h = o.out_stride_h;
+  c.lse = o.lse;
+  c.lse_stride_t = o.lse_stride_b;
+  c.num_tokens = o.batch;
+  c.num_groups = a->num_groups;
+  c.query_len = o.batch;
+  c.num_q_heads = o.num_q_heads;
+  c.num_kv_heads = o.num_kv_heads;
+  c.head_dim = o.head_dim;
+  c.page_size = o.page_size;
+  c.max_pages_per_seq = a->prefix_max_pages;
+  c.q_dtype = o.q_dtype;
+  c.kv_dtype = o.kv_dtype;
+  c.softmax_scale = o.softmax_scale;
+  c.workspace = o.workspace;
+  c.workspace_bytes = o.workspace_bytes;
+  c.num_ctas = o.num_ctas;
+  c.flags = o.flags & B2D_FLAG_TEST_NO_LOADS;
+  c.kv_layout = o.kv_layout;
+  c.wait_limit_us = o.wait_limit_us;
+  return c;
+}
+
+struct SharedLayout {
+  size_t gqa, off_part, off_pre_o, off_pre_lse, off_own_o, off_own_lse, bytes;
+};
+
+static int shared_layout(const b2d_shared_prefix_args* a, const b2d_cross_args* c,
+                         RaggedPlan* pl, SharedLayout* lay) {
+  int rc = b2d_gqa_workspace_bytes(&a->own, &lay->gqa);
+  if (rc) return rc;
+  if (a->num_groups > kMaxGroups) return B2D_ERR_TOO_LARGE;
+  if ((rc = check_sizes(c)) || (rc = make_plan(c, pl))) return rc;
+  const size_t rows = (size_t)a->own.batch * a->own.num_q_heads;
+  lay->off_part = align_up(lay->gqa, 256);
+  lay->off_pre_lse = align_up(lay->off_part + pl->bytes, 256);
+  lay->off_own_lse = align_up(lay->off_pre_lse + rows * 4, 256);
+  lay->off_pre_o = align_up(lay->off_own_lse + rows * 4, 256);
+  lay->off_own_o = align_up(lay->off_pre_o + rows * a->own.head_dim * 4, 256);
+  lay->bytes = align_up(lay->off_own_o + rows * a->own.head_dim * 4, 256);
+  return B2D_OK;
+}
+
+}  // namespace b2d
+
+using namespace b2d;
+
+extern "C" int b2d_cross_workspace_bytes(const b2d_cross_args* a, size_t* bytes) {
+  int rc = check_sizes(a);
+  if (rc) return rc;
+  if (!bytes) return B2D_ERR_INVALID_ARG;
+  RaggedPlan pl{};
+  if ((rc = make_plan(a, &pl))) return rc;
+  *bytes = kWsHeaderBytes + pl.bytes;
+  return B2D_OK;
+}
+
+extern "C" int b2d_cross_attention(const b2d_cross_args* a, void* stream) {
+  int rc = check_sizes(a);
+  if (rc) return rc;
+  if (a->num_tokens == 0 || a->num_groups == 0) return B2D_OK;
+  RaggedPlan pl{};
+  if ((rc = make_plan(a, &pl))) return rc;
+  if ((rc = check_pointers(a))) return rc;
+  if (!a->workspace || a->workspace_bytes < kWsHeaderBytes + pl.bytes) return B2D_ERR_WORKSPACE;
+  if ((uintptr_t)a->workspace & 255) return B2D_ERR_ALIGNMENT;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* part = static_cast<uint8_t*>(a->workspace) + kWsHeaderBytes;
+  for (int g0 = 0; g0 < a->num_groups; g0 += kMaxGroups) {
+    b2d_cross_args s = *a;
+    s.num_groups = std::min(a->num_groups - g0, kMaxGroups);
+    s.kv_lens = a->kv_lens + g0;
+    s.block_table = a->block_table + (int64_t)g0 * a->block_table_stride;
+    if (a->query_starts) {
+      s.query_starts = a->query_starts + g0;
+    } else {
+      const int64_t t0 = (int64_t)g0 * a->query_len;
+      s.q = static_cast<const uint8_t*>(a->q) + t0 * a->q_stride_t * 2;
+      s.out = static_cast<uint8_t*>(a->out) + t0 * a->out_stride_t * 2;
+      s.lse = a->lse ? a->lse + t0 * a->lse_stride_t : nullptr;
+      s.num_tokens = s.num_groups * a->query_len;
+    }
+    const RaggedParams p = params_of(&s, pl, part);
+    if ((rc = launch_attention(&s, pl, p, st))) return rc;
+    B2D_BY_DIM_AND_TYPE(launch_merge, a->head_dim, a->q_dtype == B2D_BF16, pl, p, st);
+    if (cudaGetLastError() != cudaSuccess) return B2D_ERR_CUDA;
+  }
+  return B2D_OK;
+}
+
+extern "C" int b2d_shared_prefix_workspace_bytes(const b2d_shared_prefix_args* a, size_t* bytes) {
+  if (!a || !bytes || a->num_groups < 0 || a->prefix_max_pages <= 0) return B2D_ERR_INVALID_ARG;
+  const b2d_cross_args c = prefix_of(a);
+  RaggedPlan pl{};
+  SharedLayout lay{};
+  const int rc = shared_layout(a, &c, &pl, &lay);
+  if (rc) return rc;
+  *bytes = lay.bytes;
+  return B2D_OK;
+}
+
+extern "C" int b2d_decode_shared_prefix(const b2d_shared_prefix_args* a, void* stream) {
+  if (!a || a->num_groups < 0 || a->prefix_max_pages <= 0) return B2D_ERR_INVALID_ARG;
+  if (a->own.flags & ~B2D_FLAG_TEST_NO_LOADS) return B2D_ERR_INVALID_ARG;
+  if (!a->group_starts && a->num_groups > 1) return B2D_ERR_INVALID_ARG;
+  const b2d_cross_args c = prefix_of(a);
+  RaggedPlan pl{};
+  SharedLayout lay{};
+  int rc = shared_layout(a, &c, &pl, &lay);
+  if (rc) return rc;
+  if (a->own.batch == 0) return B2D_OK;
+  if (a->num_groups == 0) return b2d_decode_gqa(&a->own, stream);
+  if ((rc = check_pointers(&c))) return rc;
+  if (!a->own.workspace || a->own.workspace_bytes < lay.bytes) return B2D_ERR_WORKSPACE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(a->own.workspace);
+  float* own_o = reinterpret_cast<float*>(ws + lay.off_own_o);
+  float* own_lse = reinterpret_cast<float*>(ws + lay.off_own_lse);
+  // Own tokens first: that call checks the rest of the arguments before it
+  // enqueues anything.  Its part stays in fp32; out is rounded once, by the join.
+  b2d_gqa_args own = a->own;
+  own.out = own_o;
+  own.out_stride_b = (int64_t)own.num_q_heads * own.head_dim;
+  own.out_stride_h = own.head_dim;
+  own.lse = own_lse;
+  own.lse_stride_b = own.num_q_heads;
+  own.workspace_bytes = lay.gqa;
+  if ((rc = gqa_decode_f32(&own, own_o, stream))) return rc;
+  RaggedParams p = params_of(&c, pl, ws + lay.off_part);
+  p.out_f32 = reinterpret_cast<float*>(ws + lay.off_pre_o);
+  p.lse2 = reinterpret_cast<float*>(ws + lay.off_pre_lse);
+  if ((rc = launch_attention(&c, pl, p, st))) return rc;
+  B2D_BY_DIM_AND_TYPE(launch_join, c.head_dim, c.q_dtype == B2D_BF16, pl, p, own_o, own_lse, st);
+  return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+}

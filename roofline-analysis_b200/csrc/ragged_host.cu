@@ -6,6 +6,7 @@
 #include "host_common.h"
 #include "ragged.cuh"
 #include "ragged_mma_kernel.cuh"
+#include "ragged_tc_kernel.cuh"
 
 namespace b2d {
 
@@ -14,7 +15,9 @@ namespace b2d {
 constexpr int kMaxGroups = 4096;
 
 struct RaggedPlan {
-  int TS, CH, rows, threads, ctas;
+  bool tc;       // tcgen05 kernel; else warp-level tiles
+  int granule;   // tc: keys per TMA box
+  int TS, CH, rows, ctas;
   size_t smem;
   size_t off_table, off_seg_lse, off_seg_o, bytes;  // offsets from the plan's part of the workspace
 };
@@ -64,16 +67,25 @@ static int check_pointers(const b2d_cross_args* a) {
 static int make_plan(const b2d_cross_args* a, RaggedPlan* pl) {
   const int grp = a->num_q_heads / a->num_kv_heads;
   const int groups = std::min(a->num_groups, kMaxGroups);
-  pl->rows = 64;
-  pl->threads = 128;
-  pl->CH = a->head_dim <= 128 ? 64 : 32;
-  pl->TS = pl->rows / grp;
-  pl->smem = (size_t)(pl->rows + 2 * pl->CH) * (a->head_dim + 8) * 2 + (size_t)(groups + 1) * 4 + 128;
+  pl->tc = (a->head_dim == 64 || a->head_dim == 128) && a->page_size % 16 == 0 &&
+           a->kv_layout == B2D_KV_STRIDED;
+  if (pl->tc) {
+    pl->granule = 16;   // the largest power of two up to 128 that divides a page
+    while (pl->granule < 128 && a->page_size % (2 * pl->granule) == 0) pl->granule *= 2;
+    pl->rows = 256;
+    pl->CH = 128;
+    pl->TS = 2 * (128 / grp);
+  } else {
+    pl->rows = 64;
+    pl->CH = a->head_dim <= 128 ? 64 : 32;
+    pl->TS = pl->rows / grp;
+    pl->smem = (size_t)(pl->rows + 2 * pl->CH) * (a->head_dim + 8) * 2 + (size_t)(groups + 1) * 4 + 128;
+  }
   pl->ctas = a->num_ctas;
   if (pl->ctas <= 0) {
     int sms = 0;
     if (device_sm_count(&sms) != 0) return B2D_ERR_CUDA;
-    pl->ctas = 2 * sms;
+    pl->ctas = pl->tc ? sms : 2 * sms;
   }
   // Positions on the chunk line are 32-bit in the kernels.
   const int64_t chunks = ((int64_t)a->max_pages_per_seq * a->page_size + pl->CH - 1) / pl->CH;
@@ -145,8 +157,48 @@ template <int D, int KIND, typename QT>
 static int launch_mma(const RaggedPlan& pl, const RaggedParams& p, cudaStream_t st) {
   auto kern = ragged_mma_kernel<D, KIND, QT>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), pl.smem)) return B2D_ERR_CUDA;
-  kern<<<pl.ctas, pl.threads, pl.smem, st>>>(p);
+  kern<<<pl.ctas, 128, pl.smem, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+}
+
+// {column, key of the page, head, page}: a box is `granule` keys of 128 bytes
+// (one column block, 128-byte swizzle), or of a whole e4m3 row (no swizzle;
+// the conversion writes the swizzled tile).
+static int encode_cache(CUtensorMap* map, const void* base, const b2d_cross_args* a, int granule,
+                        int64_t s_page, int64_t s_tok, int64_t s_head) {
+  const bool f8 = a->kv_dtype == B2D_FP8_E4M3;
+  const uint64_t es = f8 ? 1 : 2;
+  const uint64_t dims[4] = {(uint64_t)a->head_dim, (uint64_t)a->page_size, (uint64_t)a->num_kv_heads,
+                            (uint64_t)a->num_pages};
+  const uint64_t strides[3] = {(uint64_t)s_tok * es, (uint64_t)s_head * es, (uint64_t)s_page * es};
+  const uint32_t box[4] = {f8 ? (uint32_t)a->head_dim : 64u, (uint32_t)granule, 1u, 1u};
+  return encode_tiled_map(map, f8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4,
+                          base, dims, strides, box,
+                          f8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int D, int KIND, typename QT>
+static int launch_tc(const b2d_cross_args* a, const RaggedPlan& pl, const RaggedParams& p,
+                     cudaStream_t st) {
+  using C = RaggedTc<D, KIND>;
+  CUtensorMap tk, tv;
+  if (encode_cache(&tk, a->k_cache, a, pl.granule, a->k_stride_page, a->k_stride_tok, a->k_stride_head) ||
+      encode_cache(&tv, a->v_cache, a, pl.granule, a->v_stride_page, a->v_stride_tok, a->v_stride_head))
+    return B2D_ERR_CUDA;
+  auto kern = ragged_tc_kernel<D, KIND, QT>;
+  const size_t smem = C::smem(p.G);
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return B2D_ERR_CUDA;
+  kern<<<pl.ctas, C::kThreads, smem, st>>>(tk, tv, p, pl.granule);
+  return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+}
+
+template <int D, int KIND, typename QT>
+static int launch_one(const b2d_cross_args* a, const RaggedPlan& pl, const RaggedParams& p,
+                      cudaStream_t st) {
+  if constexpr (D <= 128) {
+    if (pl.tc) return launch_tc<D, KIND, QT>(a, pl, p, st);
+  }
+  return launch_mma<D, KIND, QT>(pl, p, st);
 }
 
 template <int D>
@@ -154,10 +206,10 @@ static int launch_attention(const b2d_cross_args* a, const RaggedPlan& pl, const
                             cudaStream_t st) {
   const bool bf = a->q_dtype == B2D_BF16;
   if (a->kv_dtype == B2D_FP8_E4M3)
-    return bf ? launch_mma<D, kKvFp8, __nv_bfloat16>(pl, p, st)
-              : launch_mma<D, kKvFp8, __half>(pl, p, st);
-  return bf ? launch_mma<D, kKvBf16, __nv_bfloat16>(pl, p, st)
-            : launch_mma<D, kKvFp16, __half>(pl, p, st);
+    return bf ? launch_one<D, kKvFp8, __nv_bfloat16>(a, pl, p, st)
+              : launch_one<D, kKvFp8, __half>(a, pl, p, st);
+  return bf ? launch_one<D, kKvBf16, __nv_bfloat16>(a, pl, p, st)
+            : launch_one<D, kKvFp16, __half>(a, pl, p, st);
 }
 
 static int launch_attention(const b2d_cross_args* a, const RaggedPlan& pl, const RaggedParams& p,

@@ -439,7 +439,7 @@ def test_merge_states_strided_in_place_of_decode(cuda):
     assert (wide[..., :64] == 0).all() and (wide[..., 192:] == 0).all()
 
 
-def _test_wait_timeout_is_reported(cuda):
+def test_wait_timeout_is_reported(cuda):
     """With the loads left out every bounded wait runs out; the call reports
     it, and the next call on the same workspace is right."""
     gen, k, v, _, _, bt = make(cuda, 190, [600, 300], 16, 2, 128, BF, "NHD")

@@ -13,14 +13,17 @@
 // tile's rows are (token, head of the KV head) pairs: row r is token r / grp,
 // head h * grp + r % grp.  A tile takes TS whole tokens, TS * grp <= its rows.
 //
-// Work split.  An item is (group, KV head, TS tokens); it has ceil(kv_len /
-// CH) chunks of CH keys.  The chunks of all items form one line, cut into
-// equal ranges, one per CTA (as the decode kernel does), so few long items
-// fill the GPU as well as many short ones.  Within a group the token tiles
-// of one KV head are neighbours on the line, so they read its K and V at
-// about the same time, from L2.  An item inside one range is written
-// directly; the pieces of a cut item go to the segments of their CTAs (a
-// range cuts at most its first and its last item: two segments per CTA).
+// Work split.  An item is one tile of one KV head of a group, or two that run
+// side by side (pairs = 1, the tcgen05 kernel): two neighbouring tiles of a
+// KV head, which share its K and V, and, for the odd last tile, the same
+// tile of two neighbouring KV heads.  An item has ceil(kv_len / CH) chunks of
+// CH keys.  The chunks of all items form one line, cut into equal ranges, one
+// per CTA (as the decode kernel does), so few long items fill the GPU as well
+// as many short ones.  Within a group the tiles of one KV head are neighbours
+// on the line, so they read its K and V at about the same time, from L2.  An
+// item inside one range is written directly; the pieces of a cut item go to
+// the segments of their CTAs (a range cuts at most its first and its last
+// item: two segments per CTA).
 #pragma once
 
 #include "common.cuh"
@@ -56,7 +59,8 @@ struct RaggedParams {
   unsigned long long wait_ns;
   int no_loads;
   int G, T, uniform, Hq, Hkv, grp, P, num_pages, max_pages;
-  int TS, CH, rows;             // tokens and rows of an item, keys of a chunk
+  int TS, CH, rows;             // tokens of a tile, keys of a chunk, rows of a segment
+  int pairs;                    // 1: items of two tiles
   float scale;                  // softmax_scale * log2(e)
 };
 
@@ -80,6 +84,12 @@ __device__ __forceinline__ int ragged_kv_len(const RaggedParams& p, int g) {
   return n < 0 ? 0 : (n > cap ? cap : n);
 }
 
+// Items of a group with n tokens.
+__device__ __forceinline__ int ragged_items(const RaggedParams& p, int n) {
+  const int tiles = (n + p.TS - 1) / p.TS;
+  return p.pairs ? p.Hkv * (tiles >> 1) + (tiles & 1) * ((p.Hkv + 1) >> 1) : p.Hkv * tiles;
+}
+
 // table[g] = chunks of all items before group g (block-wide scan; ends with
 // __syncthreads).  warp_tmp: 32 ints.
 __device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* table,
@@ -91,8 +101,7 @@ __device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* tab
     const int g = base + tid;
     int n = 0;
     if (g < p.G) {
-      const int tiles = (ragged_tokens(p, g).y + p.TS - 1) / p.TS;
-      n = p.Hkv * tiles * ((ragged_kv_len(p, g) + p.CH - 1) / p.CH);
+      n = ragged_items(p, ragged_tokens(p, g).y) * ((ragged_kv_len(p, g) + p.CH - 1) / p.CH);
     }
     int x = n;
 #pragma unroll
@@ -122,9 +131,14 @@ __device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* tab
 }
 
 // The piece of an item that starts at line position x, inside a range that
-// ends at x1.
+// ends at x1: chunks [c0, c1) of nch.  Part s (0 or 1) of the item is the
+// tile of TS tokens from tile + (tiles == 2 ? s : 0) on, of KV head h +
+// (heads == 2 ? s : 0); it exists for s < tiles * heads.
 struct RaggedPiece {
-  int g, h, t0, ntok, len, c0, c1, nch;  // ntok: tokens of the item; chunks [c0, c1) of nch
+  int g, h, tile, tiles, heads, t0, n, len, c0, c1, nch;   // group's tokens: [t0, t0 + n)
+  __device__ __forceinline__ int parts() const { return tiles * heads; }
+  __device__ __forceinline__ int head(int s) const { return h + (heads == 2 ? s : 0); }
+  __device__ __forceinline__ int first(int s, int TS) const { return (tile + (tiles == 2 ? s : 0)) * TS; }
 };
 
 __device__ __forceinline__ RaggedPiece ragged_piece(const RaggedParams& p, const int32_t* table,
@@ -132,6 +146,8 @@ __device__ __forceinline__ RaggedPiece ragged_piece(const RaggedParams& p, const
   RaggedPiece w;
   w.g = g;
   const int2 tok = ragged_tokens(p, g);
+  w.t0 = tok.x;
+  w.n = tok.y;
   w.len = ragged_kv_len(p, g);
   w.nch = (w.len + p.CH - 1) / p.CH;
   const int tiles = (tok.y + p.TS - 1) / p.TS;
@@ -139,11 +155,30 @@ __device__ __forceinline__ RaggedPiece ragged_piece(const RaggedParams& p, const
   const int it = rel / w.nch;
   w.c0 = rel - it * w.nch;
   w.c1 = min(w.nch, w.c0 + (x1 - x));
-  w.h = it / tiles;
-  const int tile = it - w.h * tiles;
-  w.t0 = tok.x + tile * p.TS;
-  w.ntok = min(p.TS, tok.y - tile * p.TS);
+  const int per = p.pairs ? tiles >> 1 : tiles;   // items of a KV head
+  w.tiles = p.pairs ? 2 : 1;
+  w.heads = 1;
+  if (it < p.Hkv * per) {
+    w.h = it / per;
+    w.tile = (it - w.h * per) * w.tiles;
+  } else {
+    w.h = 2 * (it - p.Hkv * per);
+    w.tile = tiles - 1;
+    w.tiles = 1;
+    w.heads = min(2, p.Hkv - w.h);
+  }
   return w;
+}
+
+// Where token i of a group of n and query head h are: item and row of its
+// segments.
+__device__ __forceinline__ int2 ragged_row(const RaggedParams& p, int n, int i, int h) {
+  const int tiles = (n + p.TS - 1) / p.TS, tile = i / p.TS, kvh = h / p.grp;
+  const int r = (i - tile * p.TS) * p.grp + (h - kvh * p.grp);
+  if (!p.pairs) return make_int2(kvh * tiles + tile, r);
+  const int per = tiles >> 1;
+  if (tile < 2 * per) return make_int2(kvh * per + (tile >> 1), (tile & 1) * p.TS * p.grp + r);
+  return make_int2(p.Hkv * per + (kvh >> 1), (kvh & 1) * p.TS * p.grp + r);
 }
 
 __device__ __forceinline__ int range_begin(int64_t W, int ctas, int c) {
@@ -239,10 +274,13 @@ __global__ void __launch_bounds__(256) ragged_merge_kernel(const RaggedParams p,
   const int xs = b - w.c0;
   if (w.c0 == 0 || xs < range_begin(W, ctas, c)) return;  // not cut here, or owned by an earlier CTA
   const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < w.ntok * p.grp; r += gridDim.y * 8) {
+  const int per = p.TS * p.grp;   // rows of a part
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < w.parts() * per; r += gridDim.y * 8) {
+    const int s = r / per, i = w.first(s, p.TS) + (r - s * per) / p.grp;
+    if (i >= w.n) continue;
     StateMerge<EPL> m;
     merge_segments<D>(p, W, ctas, xs, xs + w.nch, r, m);
-    const int t = w.t0 + r / p.grp, h = w.h * p.grp + r % p.grp;
+    const int t = w.t0 + i, h = w.head(s) * p.grp + r % p.grp;
     store_lane<EPL>(reinterpret_cast<QT*>(p.out) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh +
                         lane * EPL, m.acc, m.inv());
     if (p.lse != nullptr && lane == 0) p.lse[(int64_t)t * p.lse_st + h] = m.lse2() * kLn2;
@@ -276,15 +314,15 @@ __global__ void __launch_bounds__(256) shared_join_kernel(const RaggedParams p, 
   if (t >= tok.x && t < tok.x + tok.y && len > 0) {
     const int W = p.table_g[p.G];
     if (W < ctas) ctas = W;
-    const int nch = (len + p.CH - 1) / p.CH, tiles = (tok.y + p.TS - 1) / p.TS;
-    const int i = t - tok.x, kvh = h / p.grp;
-    const int xs = p.table_g[lo] + (kvh * tiles + i / p.TS) * nch;
+    const int nch = (len + p.CH - 1) / p.CH;
+    const int2 at = ragged_row(p, tok.y, t - tok.x, h);
+    const int xs = p.table_g[lo] + at.x * nch;
     if (cta_of_chunk(xs, W, ctas) == cta_of_chunk(xs + nch - 1, W, ctas)) {
       float o[EPL];
       load_lane<EPL>(p.out_f32 + row * D + lane * EPL, o);
       m.add(o, p.lse2[row]);
     } else {
-      merge_segments<D>(p, W, ctas, xs, xs + nch, (i % p.TS) * p.grp + h % p.grp, m);
+      merge_segments<D>(p, W, ctas, xs, xs + nch, at.y, m);
     }
   }
   float o[EPL];

@@ -74,7 +74,7 @@ static int make_plan(const b2d_cross_args* a, RaggedPlan* pl) {
     while (pl->granule < 128 && a->page_size % (2 * pl->granule) == 0) pl->granule *= 2;
     pl->rows = 256;
     pl->CH = 128;
-    pl->TS = 2 * (128 / grp);
+    pl->TS = 128 / grp;
   } else {
     pl->rows = 64;
     pl->CH = a->head_dim <= 128 ? 64 : 32;
@@ -149,6 +149,7 @@ static RaggedParams params_of(const b2d_cross_args* a, const RaggedPlan& pl, uin
   p.TS = pl.TS;
   p.CH = pl.CH;
   p.rows = pl.rows;
+  p.pairs = pl.tc ? 1 : 0;
   p.scale = a->softmax_scale * 1.4426950408889634f;
   return p;
 }

@@ -75,13 +75,13 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
   for (int x = x0; x < x1;) {
     while (x >= table[g + 1]) ++g;
     const RaggedPiece w = ragged_piece(p, table, g, x, x1);
-    const int nrows = w.ntok * p.grp;
+    const int t0 = w.t0 + w.first(0, p.TS), nrows = min(p.TS, w.n - w.first(0, p.TS)) * p.grp;
     __syncthreads();
     for (int i = tid; i < C::kRows * (D / 8); i += 128) {
       const int r = i / (D / 8), c = (i - r * (D / 8)) * 8;
       uint32_t o[4] = {0, 0, 0, 0};
       if (r < nrows) {
-        const QT* src = reinterpret_cast<const QT*>(p.q) + (int64_t)(w.t0 + r / p.grp) * p.q_st +
+        const QT* src = reinterpret_cast<const QT*>(p.q) + (int64_t)(t0 + r / p.grp) * p.q_st +
                         (int64_t)(w.h * p.grp + r % p.grp) * p.q_sh + c;
         float f[8];
         load_q8<QT>(src, f);
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
       if (row >= nrows) continue;
       const float inv = l[r] > 0.f ? vscale / l[r] : l[r];   // no mass at all: 0; NaN stays
       const float lse2 = m[r] + fast_log2(l[r]);
-      const int t = w.t0 + row / p.grp, h = w.h * p.grp + row % p.grp;
+      const int t = t0 + row / p.grp, h = w.h * p.grp + row % p.grp;
       if (whole && p.out_f32 == nullptr) {
         QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 2 * tq;
 #pragma unroll

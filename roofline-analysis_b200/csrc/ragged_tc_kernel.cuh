@@ -14,18 +14,17 @@
 // their own.
 //
 // Warps 0-3 and 4-7: softmax and output of stream 0 and 1 (thread = row =
-// TMEM lane, so maximum, sum and rescaling need no other thread).  Warps 8 and
-// 9: the MMAs of stream 0 and 1, so that neither stream waits for the other's
-// softmax; the tensor cores take what is there.  Warp 10: TMA.  Warp 11: the
-// last V tile of a sequence, see below.  e4m3 caches: warps 12-15 convert each
-// raw tile to fp16 (exact) into the swizzled layout the MMAs read; q and P are
-// then fp16 too.  The softmax warps get registers of the others (setmaxnreg).
+// TMEM lane, so maximum, sum and rescaling need no other thread).  Warp 8:
+// one thread issues the MMAs of both streams in turn, which keeps one stream's
+// products beside the other's softmax.  Warp 10: TMA.  Warp 11: the last V
+// tile of a sequence, see below.  e4m3 caches: warps 12-15 convert each raw
+// tile to fp16 (exact) into the swizzled layout the MMAs read; q and P are then
+// fp16 too.  The softmax warps get registers of the others (setmaxnreg).
 //
 // The maximum is lazy: it moves only when a score exceeds it by 2^8, so P <=
 // 256 and O is rescaled (a TMEM round trip) rarely.  So the weights are
 // computed with the old maximum at once, while the chunk's own maximum is
-// found beside them, and computed again in the rare case that it moves.  The
-// first 64 keys of P are handed to P.V while the rest is computed.
+// found beside them, and computed again in the rare case that it moves.
 //
 // Keys past the end: their pages are not loaded, their scores are masked, and
 // warp 11 (e4m3: the conversion) zeroes their V rows, which may hold anything,
@@ -60,8 +59,8 @@ struct RaggedTc {
   static constexpr uint32_t kOffRaw = kOffRing + kSlots * kTile;
   static constexpr uint32_t kOffStage = kOffRaw + kRawSlots * kRaw;
   static constexpr uint32_t kOffBar = kOffStage + 8 * kStage;
-  // full, empty, tail [slots]; raw full, empty; q, s, half p, p, o full [2]; drain [2]
-  static constexpr int kBars = 3 * kSlots + 2 * kRawSlots + 12;
+  // full, empty, tail [slots]; raw full, empty; q, s, p, o full [2]; drain
+  static constexpr int kBars = 3 * kSlots + 2 * kRawSlots + 9;
   static constexpr uint32_t kOffTmem = kOffBar + kBars * 8;
   static constexpr uint32_t kOffTable = kOffTmem + 16;
   static constexpr size_t smem(int groups) { return kOffTable + (size_t)(groups + 1 + 32) * 4 + 1024; }
@@ -145,8 +144,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   uint64_t* raw_empty = raw_full + NR;
   uint64_t* q_full = raw_empty + NR;
   uint64_t* s_full = q_full + 2;
-  uint64_t* p_half = s_full + 2;   // the first 64 keys of P are written
-  uint64_t* p_full = p_half + 2;
+  uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffTmem);
@@ -156,7 +154,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(full + i, F8 ? 4 : 1);
-      mbar_init(empty + i, 2);      // both streams
+      mbar_init(empty + i, 1);
       mbar_init(tail + i, 1);
     }
     for (int i = 0; i < NR; ++i) {
@@ -166,11 +164,10 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(q_full + s, 4);
       mbar_init(s_full + s, 1);
-      mbar_init(p_half + s, 4);
       mbar_init(p_full + s, 4);
       mbar_init(o_full + s, 1);
-      mbar_init(drain + s, 1);
     }
+    mbar_init(drain, 1);
     fence_barrier_init();
   }
   if (warp == 8) {
@@ -335,25 +332,16 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           tmem_wait_ld();
           weights(v, off, pk, sum, nvalid - c);
           tmem_st16(t_s + (uint32_t)(c >> 1), pk);
-          if (c == 32) {
-            tmem_wait_st();
-            tc_fence_before();
-            arrive(p_half + st);
-          }
         }
         l += sum.x + sum.y;
       };
       // The usual step: no masked key, and no maximum that has to move.
       // False: nothing was done.
       auto fast_step = [&]() -> bool {
-        uint32_t v[CH], pk[32];
+        uint32_t v[CH];
 #pragma unroll
         for (int c = 0; c < CH; c += 32) tmem_ld32(t_s + (uint32_t)c, v + c);
         tmem_wait_ld();
-        const float off = -m * sl;
-        float2 s0 = make_float2(0.f, 0.f), s1 = s0;
-        weights(v, off, pk, s0);
-        weights(v + 32, off, pk + 16, s1);
         float mc[4] = {m, m, m, m};
 #pragma unroll
         for (int j = 0; j < CH; j += 8)
@@ -363,17 +351,14 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
         const float cm = max3_nan(mc[0], mc[1], max3_nan(mc[2], mc[3], m));
         // (a NaN, or infinities on either side, fail this too)
         if (!__all_sync(0xffffffffu, (cm - m) * sl <= kLazy)) return false;
-        tmem_st16(t_s, pk);
-        tmem_st16(t_s + 16u, pk + 16);
-        tmem_wait_st();
-        tc_fence_before();
-        arrive(p_half + st);
+        const float off = -m * sl;
+        float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
-        for (int j = 64; j < CH; ++j) asm volatile("" : "+r"(v[j]));   // the rest comes after it
-        weights(v + 64, off, pk, s0);
-        weights(v + 96, off, pk + 16, s1);
-        tmem_st16(t_s + 32u, pk);
-        tmem_st16(t_s + 48u, pk + 16);
+        for (int c = 0; c < CH; c += 32) {
+          uint32_t pk[16];
+          weights(v + c, off, pk, (c & 32) ? s1 : s0);
+          tmem_st16(t_s + (uint32_t)(c >> 1), pk);
+        }
         l += (s0.x + s0.y) + (s1.x + s1.y);
         return true;
       };
@@ -386,9 +371,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
         if (live) {
           if (i == 0 || nvalid < CH || !fast_step()) full_step(i, nvalid);
           tmem_wait_st();
-        } else {
-          arrive(p_half + st);                   // rows that do not exist: P is never used
-        }
+        }                                        // (rows that do not exist: P is never used)
         tc_fence_before();
         arrive(p_full + st);
       }
@@ -478,86 +461,67 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   }
   // The ring holds, for each chunk of a piece and each KV head of its item, K
   // and then V: `heads` pairs of slots per chunk.
-  if (warp == 8 || warp == 9) {
-    // ---------------- MMAs of one stream ----------------
-    constexpr uint32_t idesc_qk = umma_idesc_16(BF, 128, CH, false);
-    constexpr uint32_t idesc_pv = umma_idesc_16(BF, 128, D, true);
-    const int st = warp - 8;
-    const uint32_t ts = tmem + (uint32_t)(st * 128), to = tmem + 256u + (uint32_t)(st * D);
-    const uint64_t qd = umma_desc_sw128(sbase + C::kOffQ + (uint32_t)st * C::kTile, 16, 1024);
-    uint32_t ring = 0;                           // ring position of the piece's first K
-    uint32_t np = 0, nq = 0;
-    int g = g_first;
-    bool ok = true;
-    for (int x = x0; x < x1 && ok;) {
-      while (x >= table[g + 1]) ++g;
-      const RaggedPiece w = ragged_piece(p, table, g, x, x1);
-      const int nc = w.c1 - w.c0;
-      const bool mine = st < w.parts();
-      const int steps = mine ? nc : 0;
-      const uint32_t own = ring + (w.heads == 2 ? 2u * (uint32_t)st : 0u);   // this stream's first K
-      x += nc;
-      // Both streams go through every ring slot, so that neither falls two
-      // phases of a barrier behind: tiles of the other stream are passed.
-      auto pass = [&](uint32_t n) -> bool {
-        for (uint32_t e = n + 2u; n < e; ++n) {
-          if (!wait(full + n % NS, (n / NS) & 1u)) return false;
-          arrive(empty + n % NS);
-        }
-        return true;
+  if (warp == 8) {
+    // ---------------- MMAs (one thread) ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc_qk = umma_idesc_16(BF, 128, CH, false);
+      constexpr uint32_t idesc_pv = umma_idesc_16(BF, 128, D, true);
+      auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
+        for (int i = 0; i < 64; ++i)
+          if (mbar_try_wait(bar, parity)) return true;
+        return mla_wait(bar, parity, p.status, p.wait_ns);
       };
-      for (int i = 0; i <= steps && ok && steps > 0; ++i) {
-        if (i > 0) {                             // O += P.V of step i - 1
-          const uint32_t n = own + (uint32_t)(2 * w.heads * (i - 1)) + 1u, slot = n % NS;
-          ok = wait(full + slot, (n / NS) & 1u) && wait(p_half + st, np & 1u);
-          if (!ok) break;
+      uint32_t ring = 0;                         // ring position of the piece's first K
+      uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
+      int g = g_first;
+      bool ok = true;
+      for (int x = x0; x < x1 && ok;) {
+        while (x >= table[g + 1]) ++g;
+        const RaggedPiece w = ragged_piece(p, table, g, x, x1);
+        const int nc = w.c1 - w.c0, parts = w.parts();
+        x += nc;
+        // Ring position of stream st's K of chunk i; whether the stream is the
+        // tile's last reader.
+        auto k_at = [&](int st, int i) { return ring + (uint32_t)(2 * (w.heads * i + (w.heads == 2 ? st : 0))); };
+        auto last = [&](int st) { return w.heads == 2 || st == parts - 1; };
+        auto qk = [&](int st, int i) -> bool {   // S of step i
+          const uint32_t n = k_at(st, i), slot = n % NS;
+          if (!wait1(full + slot, (n / NS) & 1u)) return false;
+          tc_fence_after();
+          const uint64_t qd = umma_desc_sw128(sbase + C::kOffQ + (uint32_t)st * C::kTile, 16, 1024);
+          const uint64_t kd = umma_desc_sw128(sbase + C::kOffRing + slot * C::kTile, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t o = (uint64_t)(((k >> 2) * 16384 + (k & 3) * 32) >> 4);
+            umma_bf16(tmem + (uint32_t)(st * 128), qd + o, kd + o, idesc_qk, k > 0);
+          }
+          umma_commit(s_full + st);
+          if (last(st)) umma_commit(empty + slot);
+          return true;
+        };
+        auto pv = [&](int st, int i) -> bool {   // O += P.V of step i
+          const uint32_t n = k_at(st, i) + 1u, slot = n % NS;
+          if (!wait1(full + slot, (n / NS) & 1u) || !wait1(p_full + st, np[st]++ & 1u)) return false;
+          tc_fence_after();
+          const uint32_t ts = tmem + (uint32_t)(st * 128), to = tmem + 256u + (uint32_t)(st * D);
           const uint64_t vd = umma_desc_sw128(sbase + C::kOffRing + slot * C::kTile, 16384, 1024);
-          tc_fence_after();
-          if (lane == 0) {
 #pragma unroll
-            for (int k = 0; k < CH / 32; ++k)
-              umma_bf16_ts(to, ts + 8u * k, vd + (uint64_t)((k * 2048) >> 4), idesc_pv, i > 1 || k > 0);
-          }
-          if (!(ok = wait(p_full + st, np & 1u))) break;
-          ++np;
-          tc_fence_after();
-          if (lane == 0) {
-#pragma unroll
-            for (int k = CH / 32; k < CH / 16; ++k)
-              umma_bf16_ts(to, ts + 8u * k, vd + (uint64_t)((k * 2048) >> 4), idesc_pv, true);
-            umma_commit(empty + slot);
-            if (i == steps) umma_commit(o_full + st);
-          }
-          __syncwarp();
-        }
-        if (i < steps) {                         // S of step i
-          const uint32_t n = own + (uint32_t)(2 * w.heads * i), slot = n % NS;
-          if (w.heads == 2 && st == 1) ok = pass(n - 2u);
-          if (i == 0) ok = ok && wait(q_full + st, nq++ & 1u);
-          ok = ok && wait(full + slot, (n / NS) & 1u);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint64_t kd = umma_desc_sw128(sbase + C::kOffRing + slot * C::kTile, 16, 1024);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint64_t o = (uint64_t)(((k >> 2) * 16384 + (k & 3) * 32) >> 4);
-              umma_bf16(ts, qd + o, kd + o, idesc_qk, k > 0);
-            }
-            umma_commit(s_full + st);
-            umma_commit(empty + slot);
-          }
-          __syncwarp();
-          if (w.heads == 2 && st == 0) ok = pass(n + 2u);
-        }
+          for (int k = 0; k < CH / 16; ++k)
+            umma_bf16_ts(to, ts + 8u * k, vd + (uint64_t)((k * 2048) >> 4), idesc_pv, i > 0 || k > 0);
+          if (last(st)) umma_commit(empty + slot);
+          if (i + 1 == nc) umma_commit(o_full + st);
+          return true;
+        };
+        for (int st = 0; st < parts && ok; ++st) ok = wait1(q_full + st, nq[st]++ & 1u) && qk(st, 0);
+        for (int i = 0; i < nc && ok; ++i)
+          for (int st = 0; st < parts && ok; ++st) ok = pv(st, i) && (i + 1 >= nc || qk(st, i + 1));
+        ring += (uint32_t)(2 * w.heads * nc);
       }
-      for (int i = 0; i < nc && ok && !mine; ++i) ok = pass(ring + 2u * (uint32_t)i);
-      ring += (uint32_t)(2 * w.heads * nc);
+      // Nothing of this thread is in flight when tensor memory is freed.
+      umma_commit(drain);
+      wait1(drain, 0);
     }
-    // Nothing of this warp is in flight when tensor memory is freed.
-    if (lane == 0) umma_commit(drain + st);
     __syncwarp();
-    wait(drain + st, 0);
   } else if (warp == 10) {
     // ---------------- TMA producer ----------------
     if (!p.no_loads) {

@@ -19,17 +19,22 @@
 // tile of two neighbouring KV heads.  An item has ceil(kv_len / CH) chunks of
 // CH keys.  The chunks of all items form one line, cut into equal ranges, one
 // per CTA (as the decode kernel does), so few long items fill the GPU as well
-// as many short ones.  Within a group the tiles of one KV head are neighbours
+// as many short ones.  On the line an item is kItemCost chunks longer than it
+// is: what its queries and outputs cost.  (48 ragged requests, 1 to 1500 keys:
+// without it the slowest CTA took 2.1 times the median.)  Within a group the tiles of one KV head are neighbours
 // on the line, so they read its K and V at about the same time, from L2.  An
 // item inside one range is written directly; the pieces of a cut item go to
 // the segments of their CTAs (a range cuts at most its first and its last
-// item: two segments per CTA).
+// item: segment 0 of a CTA is for an item that began before its range, segment
+// 1 for one that goes on behind it).
 #pragma once
 
 #include "common.cuh"
 #include "gqa_kernel.cuh"
 
 namespace b2d {
+
+constexpr int kItemCost = 1;   // positions of an item on the line before its first chunk
 
 struct RaggedParams {
   const void* q;
@@ -49,12 +54,11 @@ struct RaggedParams {
   int64_t o_st, o_sh;
   float* lse;                   // natural log; may be null
   int64_t lse_st;
-  float* out_f32;               // shared prefix: uncut items go here, [T, Hq, D] fp32, with
-                                // lse2 [T, Hq] in log2 units; null: they go to out and lse
-  float* lse2;
+  const float* own_o;           // shared prefix: the part over each sequence's own tokens, [T, Hq, D]
+  const float* own_lse;         // fp32 and [T, Hq] natural log, to be joined with; else null
   float* seg_o;                 // [2 * CTAs][tile rows][D] fp32, normalised
   float* seg_lse;               // [2 * CTAs][tile rows], log2 units
-  int32_t* table_g;             // [G + 1], written by CTA 0 for the merge
+  int32_t* cuts;                // [CTAs][8]: the item that each CTA begins and does not finish
   int* status;
   unsigned long long wait_ns;
   int no_loads;
@@ -90,7 +94,7 @@ __device__ __forceinline__ int ragged_items(const RaggedParams& p, int n) {
   return p.pairs ? p.Hkv * (tiles >> 1) + (tiles & 1) * ((p.Hkv + 1) >> 1) : p.Hkv * tiles;
 }
 
-// table[g] = chunks of all items before group g (block-wide scan; ends with
+// table[g] = line positions of all items before group g (block-wide scan; ends with
 // __syncthreads).  warp_tmp: 32 ints.
 __device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* table,
                                              int32_t* warp_tmp) {
@@ -101,7 +105,8 @@ __device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* tab
     const int g = base + tid;
     int n = 0;
     if (g < p.G) {
-      n = ragged_items(p, ragged_tokens(p, g).y) * ((ragged_kv_len(p, g) + p.CH - 1) / p.CH);
+      const int nch = (ragged_kv_len(p, g) + p.CH - 1) / p.CH;
+      n = nch > 0 ? ragged_items(p, ragged_tokens(p, g).y) * (nch + kItemCost) : 0;
     }
     int x = n;
 #pragma unroll
@@ -130,81 +135,57 @@ __device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* tab
   __syncthreads();
 }
 
-// The piece of an item that starts at line position x, inside a range that
-// ends at x1: chunks [c0, c1) of nch.  Part s (0 or 1) of the item is the
-// tile of TS tokens from tile + (tiles == 2 ? s : 0) on, of KV head h +
-// (heads == 2 ? s : 0); it exists for s < tiles * heads.
+// A piece of an item, inside one range: chunks [c0, c1) of nch.  Part s (0 or
+// 1) of the item is the tile of TS tokens from tile + (tiles == 2 ? s : 0) on,
+// of KV head h + (heads == 2 ? s : 0); it exists for s < tiles * heads.
 struct RaggedPiece {
   int g, h, tile, tiles, heads, t0, n, len, c0, c1, nch;   // group's tokens: [t0, t0 + n)
+  int last;                                                // line position of the item's last chunk
   __device__ __forceinline__ int parts() const { return tiles * heads; }
   __device__ __forceinline__ int head(int s) const { return h + (heads == 2 ? s : 0); }
   __device__ __forceinline__ int first(int s, int TS) const { return (tile + (tiles == 2 ? s : 0)) * TS; }
+  __device__ __forceinline__ bool whole() const { return c0 == 0 && c1 == nch; }
+  __device__ __forceinline__ int segment(int cta) const { return 2 * cta + (c0 == 0 ? 1 : 0); }
 };
 
-__device__ __forceinline__ RaggedPiece ragged_piece(const RaggedParams& p, const int32_t* table,
-                                                    int g, int x, int x1) {
-  RaggedPiece w;
-  w.g = g;
-  const int2 tok = ragged_tokens(p, g);
-  w.t0 = tok.x;
-  w.n = tok.y;
-  w.len = ragged_kv_len(p, g);
-  w.nch = (w.len + p.CH - 1) / p.CH;
-  const int tiles = (tok.y + p.TS - 1) / p.TS;
-  const int rel = x - table[g];
-  const int it = rel / w.nch;
-  w.c0 = rel - it * w.nch;
-  w.c1 = min(w.nch, w.c0 + (x1 - x));
-  const int per = p.pairs ? tiles >> 1 : tiles;   // items of a KV head
-  w.tiles = p.pairs ? 2 : 1;
-  w.heads = 1;
-  if (it < p.Hkv * per) {
-    w.h = it / per;
-    w.tile = (it - w.h * per) * w.tiles;
-  } else {
-    w.h = 2 * (it - p.Hkv * per);
-    w.tile = tiles - 1;
-    w.tiles = 1;
-    w.heads = min(2, p.Hkv - w.h);
+// The next piece with a chunk in line positions [x, x1); moves x behind it and
+// g to its group.  False: none is left.
+__device__ __forceinline__ bool ragged_next(const RaggedParams& p, const int32_t* table, int x1,
+                                            int& g, int& x, RaggedPiece& w) {
+  while (x < x1) {
+    while (x >= table[g + 1]) ++g;
+    w.g = g;
+    const int2 tok = ragged_tokens(p, g);
+    w.t0 = tok.x;
+    w.n = tok.y;
+    w.len = ragged_kv_len(p, g);
+    w.nch = (w.len + p.CH - 1) / p.CH;
+    const int tiles = (tok.y + p.TS - 1) / p.TS;
+    const int rel = x - table[g], size = w.nch + kItemCost;
+    const int it = rel / size, pos = rel - it * size, end = min(size, pos + (x1 - x));
+    w.c0 = max(0, pos - kItemCost);
+    w.c1 = max(0, end - kItemCost);
+    w.last = x - pos + size - 1;
+    x += end - pos;
+    const int per = p.pairs ? tiles >> 1 : tiles;   // items of a KV head
+    w.tiles = p.pairs ? 2 : 1;
+    w.heads = 1;
+    if (it < p.Hkv * per) {
+      w.h = it / per;
+      w.tile = (it - w.h * per) * w.tiles;
+    } else {
+      w.h = 2 * (it - p.Hkv * per);
+      w.tile = tiles - 1;
+      w.tiles = 1;
+      w.heads = min(2, p.Hkv - w.h);
+    }
+    if (w.c1 > w.c0) return true;
   }
-  return w;
-}
-
-// Where token i of a group of n and query head h are: item and row of its
-// segments.
-__device__ __forceinline__ int2 ragged_row(const RaggedParams& p, int n, int i, int h) {
-  const int tiles = (n + p.TS - 1) / p.TS, tile = i / p.TS, kvh = h / p.grp;
-  const int r = (i - tile * p.TS) * p.grp + (h - kvh * p.grp);
-  if (!p.pairs) return make_int2(kvh * tiles + tile, r);
-  const int per = tiles >> 1;
-  if (tile < 2 * per) return make_int2(kvh * per + (tile >> 1), (tile & 1) * p.TS * p.grp + r);
-  return make_int2(p.Hkv * per + (kvh >> 1), (kvh & 1) * p.TS * p.grp + r);
+  return false;
 }
 
 __device__ __forceinline__ int range_begin(int64_t W, int ctas, int c) {
   return (int)((int64_t)c * W / ctas);
-}
-
-// Query rows of groups without keys: out = 0, lse = -inf.
-template <int D, typename QT>
-__device__ __forceinline__ void ragged_zero_rows(const RaggedParams& p) {
-  for (int g = blockIdx.x; g < p.G; g += gridDim.x) {
-    if (ragged_kv_len(p, g) > 0) continue;
-    const int2 tok = ragged_tokens(p, g);
-    const int64_t n = (int64_t)tok.y * p.Hq;
-    for (int64_t i = threadIdx.x; i < n * (D / 8); i += blockDim.x) {
-      const int64_t row = i / (D / 8);
-      const int c = (int)(i - row * (D / 8)) * 8;
-      const int t = tok.x + (int)(row / p.Hq), h = (int)(row % p.Hq);
-      if (p.out_f32 == nullptr) {
-        *reinterpret_cast<uint4*>(reinterpret_cast<QT*>(p.out) + (int64_t)t * p.o_st +
-                                  (int64_t)h * p.o_sh + c) = make_uint4(0, 0, 0, 0);
-        if (p.lse != nullptr && c == 0) p.lse[(int64_t)t * p.lse_st + h] = -INFINITY;
-      } else if (c == 0) {
-        p.lse2[(int64_t)t * p.Hq + h] = -INFINITY;  // its out_f32 row is never read
-      }
-    }
-  }
 }
 
 // Running merge of normalised partial outputs: (o, lse in log2 units), EPL
@@ -229,109 +210,171 @@ struct StateMerge {
   __device__ __forceinline__ float lse2() const { return mx + fast_log2(sum); }  // -inf when empty
 };
 
+template <typename QT>
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+  if constexpr (std::is_same<QT, __nv_bfloat16>::value) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
 template <int EPL, typename QT>
 __device__ __forceinline__ void store_lane(QT* dst, const float* v, float s) {
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) dst[e] = QT(v[e] * s);
+  for (int e = 0; e < EPL; e += 2) {   // EPL is even: 4-byte stores
+    const uint32_t w = pack_pair<QT>(v[e] * s, v[e + 1] * s);
+    *reinterpret_cast<uint32_t*>(dst + e) = w;
+  }
 }
 
 template <int EPL>
 __device__ __forceinline__ void load_lane(const float* src, float* v) {
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) v[e] = src[e];
-}
-
-// Adds the segments of row r of the item at line positions [xs, xe) to m.
-template <int D>
-__device__ __forceinline__ void merge_segments(const RaggedParams& p, int64_t W, int ctas, int xs,
-                                               int xe, int r, StateMerge<D / 32>& m) {
-  constexpr int EPL = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int cf = cta_of_chunk(xs, W, ctas), cl = cta_of_chunk(xe - 1, W, ctas);
-  for (int c = cf; c <= cl; ++c) {
-    const int slot = (c == cf && xs > range_begin(W, ctas, c)) ? 1 : 0;
-    const int64_t at = (int64_t)(2 * c + slot) * p.rows + r;
-    float o[EPL];
-    load_lane<EPL>(p.seg_o + at * D + lane * EPL, o);
-    m.add(o, p.seg_lse[at]);
+  for (int e = 0; e < EPL; e += 2) {
+    const float2 f = *reinterpret_cast<const float2*>(src + e);
+    v[e] = f.x;
+    v[e + 1] = f.y;
   }
 }
 
-// Cross attention: writes the rows of items that a range boundary cut.  Block
-// x looks at the boundary behind CTA x; the CTA in which the item starts
-// owns it.  One warp per row.
-template <int D, typename QT>
-__global__ void __launch_bounds__(256) ragged_merge_kernel(const RaggedParams p, int ctas) {
-  constexpr float kLn2 = 0.69314718055994530942f;
-  constexpr int EPL = D / 32;
-  const int W = p.table_g[p.G];
-  if (W < ctas) ctas = W;
-  const int c = blockIdx.x;
-  if (c + 1 >= ctas) return;
-  const int b = range_begin(W, ctas, c + 1);
-  const int g = find_row(p.table_g, p.G, b);
-  const RaggedPiece w = ragged_piece(p, p.table_g, g, b, b + 1);
-  const int xs = b - w.c0;
-  if (w.c0 == 0 || xs < range_begin(W, ctas, c)) return;  // not cut here, or owned by an earlier CTA
-  const int lane = threadIdx.x & 31;
-  const int per = p.TS * p.grp;   // rows of a part
-  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < w.parts() * per; r += gridDim.y * 8) {
-    const int s = r / per, i = w.first(s, p.TS) + (r - s * per) / p.grp;
-    if (i >= w.n) continue;
-    StateMerge<EPL> m;
-    merge_segments<D>(p, W, ctas, xs, xs + w.nch, r, m);
-    const int t = w.t0 + i, h = w.head(s) * p.grp + r % p.grp;
-    store_lane<EPL>(reinterpret_cast<QT*>(p.out) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh +
-                        lane * EPL, m.acc, m.inv());
-    if (p.lse != nullptr && lane == 0) p.lse[(int64_t)t * p.lse_st + h] = m.lse2() * kLn2;
+// Weights of a normalised part (log2 sum a2) and the own part (natural log
+// sum) in their join, and the join's log2 sum.  A part without mass gets 0.
+__device__ __forceinline__ float2 join_weights(float a2, float own, float& lse2) {
+  const float b2 = own * 1.4426950408889634f, mx = fmaxf(a2, b2);
+  if (mx == -INFINITY) {
+    lse2 = a2 + b2;   // -inf, or NaN
+    return make_float2(1.f, 0.f);
   }
+  const float wa = fast_exp2(a2 - mx), wb = fast_exp2(b2 - mx), inv = 1.f / (wa + wb);
+  lse2 = mx + fast_log2(wa + wb);
+  return make_float2(wa * inv, wb * inv);
 }
 
-// Shared prefix: joins each sequence's prefix part (direct or in segments)
-// with its own tokens' part (own_o [T, Hq, D] fp32, own_lse [T, Hq] natural
-// log).  One warp per (sequence, query head).
+// A row without keys of its group: its own part alone, or out = 0, lse = -inf.
+// One warp.
 template <int D, typename QT>
-__global__ void __launch_bounds__(256) shared_join_kernel(const RaggedParams p, int ctas,
-                                                          const float* own_o,
-                                                          const float* own_lse) {
-  constexpr float kLn2 = 0.69314718055994530942f;
-  constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ void ragged_row_without_keys(const RaggedParams& p, int t, int h) {
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994530942f;
   constexpr int EPL = D / 32;
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= (int64_t)p.T * p.Hq) return;
-  const int t = (int)(row / p.Hq), h = (int)(row - (int64_t)t * p.Hq);
   StateMerge<EPL> m;
-  // The group that holds sequence t, if any: the last one that starts at or
-  // before t (empty groups that start there too come before it).
-  int lo = 0, hi = p.G - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (ragged_tokens(p, mid).x <= t) lo = mid; else hi = mid - 1;
+  if (p.own_o != nullptr) {
+    const int64_t row = (int64_t)t * p.Hq + h;
+    float o[EPL];
+    load_lane<EPL>(p.own_o + row * D + lane * EPL, o);
+    m.add(o, p.own_lse[row] * kLog2e);
   }
-  const int2 tok = ragged_tokens(p, lo);
-  const int len = ragged_kv_len(p, lo);
-  if (t >= tok.x && t < tok.x + tok.y && len > 0) {
-    const int W = p.table_g[p.G];
-    if (W < ctas) ctas = W;
-    const int nch = (len + p.CH - 1) / p.CH;
-    const int2 at = ragged_row(p, tok.y, t - tok.x, h);
-    const int xs = p.table_g[lo] + at.x * nch;
-    if (cta_of_chunk(xs, W, ctas) == cta_of_chunk(xs + nch - 1, W, ctas)) {
-      float o[EPL];
-      load_lane<EPL>(p.out_f32 + row * D + lane * EPL, o);
-      m.add(o, p.lse2[row]);
-    } else {
-      merge_segments<D>(p, W, ctas, xs, xs + nch, at.y, m);
+  store_lane<EPL>(reinterpret_cast<QT*>(p.out) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + lane * EPL,
+                  m.acc, m.inv());
+  if (p.lse != nullptr && lane == 0) p.lse[(int64_t)t * p.lse_st + h] = m.lse2() * kLn2;
+}
+
+// All rows of groups without keys, and (shared prefix) of tokens outside every
+// group, spread over the blocks and their warps.
+template <int D, typename QT>
+__device__ __forceinline__ void ragged_rows_without_keys(const RaggedParams& p) {
+  const int warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  auto rows = [&](int t0, int n, int first, int step) {
+    for (int64_t i = first; i < (int64_t)n * p.Hq; i += step)
+      ragged_row_without_keys<D, QT>(p, t0 + (int)(i / p.Hq), (int)(i % p.Hq));
+  };
+  for (int g = blockIdx.x; g < p.G; g += gridDim.x)
+    if (ragged_kv_len(p, g) == 0) {
+      const int2 tok = ragged_tokens(p, g);
+      rows(tok.x, tok.y, warp, nwarps);
+    }
+  if (p.own_o != nullptr && p.starts != nullptr) {
+    const int first = blockIdx.x * nwarps + warp, step = gridDim.x * nwarps;
+    rows(0, ragged_tokens(p, 0).x, first, step);
+    const int2 tok = ragged_tokens(p, p.G - 1);
+    rows(tok.x + tok.y, p.T - tok.x - tok.y, first, step);
+  }
+}
+
+// What CTA c leaves for the merge: nothing, or the item that it begins and
+// does not finish.
+__device__ __forceinline__ void ragged_note_cut(const RaggedParams& p, int c, const RaggedPiece* w,
+                                                int64_t W, int ctas) {
+  int v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (w != nullptr) {
+    v[0] = cta_of_chunk(w->last, W, ctas) - c + 1;
+    for (int s = 0; s < w->parts(); ++s) {
+      v[2 + 3 * s] = w->t0 + w->first(s, p.TS);
+      v[3 + 3 * s] = min(p.TS, w->n - w->first(s, p.TS));
+      v[4 + 3 * s] = w->head(s);
     }
   }
-  float o[EPL];
-  load_lane<EPL>(own_o + row * D + lane * EPL, o);
-  m.add(o, own_lse[row] * kLog2e);
-  store_lane<EPL>(reinterpret_cast<QT*>(p.out) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh +
-                      lane * EPL, m.acc, m.inv());
-  if (p.lse != nullptr && lane == 0)
-    p.lse[(int64_t)t * p.lse_st + h] = m.lse2() * kLn2;
+  for (int i = 0; i < 8; ++i) p.cuts[8 * c + i] = v[i];
+}
+
+// Joins the segments of every cut item (and its rows' own parts) into out and
+// lse.  Block x takes the item that CTA x begins; one warp per row.  The
+// weights of up to 32 segments are computed side by side by the lanes; then
+// the segments' values are loaded U at a time.
+template <int D, typename QT>
+__global__ void __launch_bounds__(256) ragged_merge_kernel(const RaggedParams p) {
+  constexpr float kLn2 = 0.69314718055994530942f;
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr int EPL = D / 32, U = 8;
+  griddep_wait();
+  const int c = blockIdx.x, lane = threadIdx.x & 31;
+  const int4 a = *reinterpret_cast<const int4*>(p.cuts + 8 * c);
+  if (a.x == 0) return;
+  const int4 b = *reinterpret_cast<const int4*>(p.cuts + 8 * c + 4);
+  const int per = p.TS * p.grp;   // rows of a part
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < 2 * per; r += gridDim.y * 8) {
+    const int s = r >= per ? 1 : 0, rr = r - s * per, i = rr / p.grp;
+    if (i >= (s ? b.z : a.w)) continue;
+    const int t = (s ? b.y : a.z) + i, h = (s ? b.w : b.x) * p.grp + rr - i * p.grp;
+    auto seg_at = [&](int j) { return (int64_t)(2 * (c + j) + (j == 0 ? 1 : 0)) * p.rows + r; };
+    float acc[EPL], mx = -INFINITY, sum = 0.f, own[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) acc[e] = own[e] = 0.f;
+    if (p.own_o != nullptr) {
+      const int64_t row = (int64_t)t * p.Hq + h;
+      load_lane<EPL>(p.own_o + row * D + lane * EPL, own);
+      mx = p.own_lse[row] * kLog2e;
+      sum = mx == -INFINITY ? 0.f : 1.f;
+      if (sum != 0.f) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) acc[e] = own[e];
+      }
+    }
+    for (int j0 = 0; j0 < a.x; j0 += 32) {
+      const float l = j0 + lane < a.x ? p.seg_lse[seg_at(j0 + lane)] : -INFINITY;
+      float nm = l;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, o));
+      nm = fmaxf(nm, mx);
+      const float w = l == -INFINITY ? 0.f : fast_exp2(l - nm);
+      const float old = mx == -INFINITY ? 0.f : fast_exp2(mx - nm);
+      sum *= old;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) acc[e] *= old;
+      mx = nm;
+      const int n = min(32, a.x - j0);
+      for (int j = 0; j < n; j += U) {
+        float v[U][EPL];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          load_lane<EPL>(p.seg_o + seg_at(j0 + min(j + u, n - 1)) * D + lane * EPL, v[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float wj = __shfl_sync(0xffffffffu, w, (j + u) & 31);
+          if (j + u >= n || wj == 0.f) continue;   // (a segment without mass may hold anything)
+          sum += wj;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) acc[e] += wj * v[u][e];
+        }
+      }
+    }
+    store_lane<EPL>(reinterpret_cast<QT*>(p.out) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh +
+                        lane * EPL, acc, sum == 0.f ? 0.f : 1.f / sum);
+    if (p.lse != nullptr && lane == 0) p.lse[(int64_t)t * p.lse_st + h] = (mx + fast_log2(sum)) * kLn2;
+  }
 }
 
 }  // namespace b2d

@@ -19,7 +19,7 @@ struct RaggedPlan {
   int granule;   // tc: keys per TMA box
   int TS, CH, rows, ctas;
   size_t smem;
-  size_t off_table, off_seg_lse, off_seg_o, bytes;  // offsets from the plan's part of the workspace
+  size_t off_cuts, off_seg_lse, off_seg_o, bytes;  // offsets from the plan's part of the workspace
 };
 
 static int check_sizes(const b2d_cross_args* a) {
@@ -88,12 +88,12 @@ static int make_plan(const b2d_cross_args* a, RaggedPlan* pl) {
     pl->ctas = pl->tc ? sms : 2 * sms;
   }
   // Positions on the chunk line are 32-bit in the kernels.
-  const int64_t chunks = ((int64_t)a->max_pages_per_seq * a->page_size + pl->CH - 1) / pl->CH;
+  const int64_t chunks = ((int64_t)a->max_pages_per_seq * a->page_size + pl->CH - 1) / pl->CH + kItemCost;
   const int64_t tiles = (int64_t)a->num_tokens / pl->TS + groups;
   if (tiles * a->num_kv_heads > (int64_t)INT32_MAX / chunks) return B2D_ERR_TOO_LARGE;
   const size_t seg_rows = (size_t)2 * pl->ctas * pl->rows;
-  pl->off_table = 0;
-  pl->off_seg_lse = align_up((size_t)(groups + 1) * 4, 256);
+  pl->off_cuts = 0;
+  pl->off_seg_lse = align_up((size_t)pl->ctas * 32, 256);
   pl->off_seg_o = align_up(pl->off_seg_lse + seg_rows * 4, 256);
   pl->bytes = align_up(pl->off_seg_o + seg_rows * a->head_dim * 4, 256);
   return B2D_OK;
@@ -131,7 +131,7 @@ static RaggedParams params_of(const b2d_cross_args* a, const RaggedPlan& pl, uin
   p.o_sh = a->out_stride_h;
   p.lse = a->lse;
   p.lse_st = a->lse_stride_t;
-  p.table_g = reinterpret_cast<int32_t*>(part + pl.off_table);
+  p.cuts = reinterpret_cast<int32_t*>(part + pl.off_cuts);
   p.seg_lse = reinterpret_cast<float*>(part + pl.off_seg_lse);
   p.seg_o = reinterpret_cast<float*>(part + pl.off_seg_o);
   p.status = static_cast<int*>(a->workspace);
@@ -154,12 +154,30 @@ static RaggedParams params_of(const b2d_cross_args* a, const RaggedPlan& pl, uin
   return p;
 }
 
+// Launch whose prologue may overlap the kernel before it on the stream (the
+// kernel itself waits for that one's end before it touches global memory).
+template <typename... P, typename... A>
+static int launch_overlapped(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+                             A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess && cudaGetLastError() == cudaSuccess
+             ? B2D_OK : B2D_ERR_CUDA;
+}
+
 template <int D, int KIND, typename QT>
 static int launch_mma(const RaggedPlan& pl, const RaggedParams& p, cudaStream_t st) {
   auto kern = ragged_mma_kernel<D, KIND, QT>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), pl.smem)) return B2D_ERR_CUDA;
-  kern<<<pl.ctas, 128, pl.smem, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+  return launch_overlapped(kern, dim3(pl.ctas), 128, pl.smem, st, p);
 }
 
 // {column, key of the page, head, page}: a box is `granule` keys of 128 bytes
@@ -189,8 +207,7 @@ static int launch_tc(const b2d_cross_args* a, const RaggedPlan& pl, const Ragged
   auto kern = ragged_tc_kernel<D, KIND, QT>;
   const size_t smem = C::smem(p.G);
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kern), smem)) return B2D_ERR_CUDA;
-  kern<<<pl.ctas, C::kThreads, smem, st>>>(tk, tv, p, pl.granule);
-  return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+  return launch_overlapped(kern, dim3(pl.ctas), C::kThreads, smem, st, tk, tv, p, pl.granule);
 }
 
 template <int D, int KIND, typename QT>
@@ -223,28 +240,28 @@ static int launch_attention(const b2d_cross_args* a, const RaggedPlan& pl, const
   }
 }
 
-template <int D, typename QT>
-static void launch_merge(const RaggedPlan& pl, const RaggedParams& p, cudaStream_t st) {
-  if (pl.ctas > 1)
-    ragged_merge_kernel<D, QT><<<dim3(pl.ctas - 1, pl.rows / 8), 256, 0, st>>>(p, pl.ctas);
+template <int D>
+static int launch_merge(const b2d_cross_args* a, const RaggedPlan& pl, const RaggedParams& p,
+                        cudaStream_t st) {
+  if (pl.ctas < 2) return B2D_OK;
+  const dim3 grid(pl.ctas - 1, (unsigned)((pl.rows + 15) / 16));
+  return a->q_dtype == B2D_BF16
+             ? launch_overlapped(ragged_merge_kernel<D, __nv_bfloat16>, grid, 256, 0, st, p)
+             : launch_overlapped(ragged_merge_kernel<D, __half>, grid, 256, 0, st, p);
 }
 
-template <int D, typename QT>
-static void launch_join(const RaggedPlan& pl, const RaggedParams& p, const float* own_o,
-                        const float* own_lse, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.T * p.Hq;
-  shared_join_kernel<D, QT><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, pl.ctas, own_o, own_lse);
+// The attention kernel and the merge of the items that its ranges cut.
+static int launch_both(const b2d_cross_args* a, const RaggedPlan& pl, const RaggedParams& p,
+                       cudaStream_t st) {
+  const int rc = launch_attention(a, pl, p, st);
+  if (rc) return rc;
+  switch (a->head_dim) {
+    case 64: return launch_merge<64>(a, pl, p, st);
+    case 128: return launch_merge<128>(a, pl, p, st);
+    case 192: return launch_merge<192>(a, pl, p, st);
+    default: return launch_merge<256>(a, pl, p, st);
+  }
 }
-
-#define B2D_BY_DIM_AND_TYPE(fn, dim, bf, ...)                                      \
-  do {                                                                             \
-    switch (dim) {                                                                 \
-      case 64: (bf) ? fn<64, __nv_bfloat16>(__VA_ARGS__) : fn<64, __half>(__VA_ARGS__); break;    \
-      case 128: (bf) ? fn<128, __nv_bfloat16>(__VA_ARGS__) : fn<128, __half>(__VA_ARGS__); break; \
-      case 192: (bf) ? fn<192, __nv_bfloat16>(__VA_ARGS__) : fn<192, __half>(__VA_ARGS__); break; \
-      default: (bf) ? fn<256, __nv_bfloat16>(__VA_ARGS__) : fn<256, __half>(__VA_ARGS__); break;  \
-    }                                                                              \
-  } while (0)
 
 // The prefix half of a shared-prefix decode as a ragged problem: the
 // sequences of a group are the tokens that read its prefix.
@@ -295,7 +312,7 @@ static b2d_cross_args prefix_of(const b2d_shared_prefix_args* a) {
 }
 
 struct SharedLayout {
-  size_t gqa, off_part, off_pre_o, off_pre_lse, off_own_o, off_own_lse, bytes;
+  size_t gqa, off_part, off_own_o, off_own_lse, bytes;
 };
 
 static int shared_layout(const b2d_shared_prefix_args* a, const b2d_cross_args* c,
@@ -306,10 +323,8 @@ static int shared_layout(const b2d_shared_prefix_args* a, const b2d_cross_args* 
   if ((rc = check_sizes(c)) || (rc = make_plan(c, pl))) return rc;
   const size_t rows = (size_t)a->own.batch * a->own.num_q_heads;
   lay->off_part = align_up(lay->gqa, 256);
-  lay->off_pre_lse = align_up(lay->off_part + pl->bytes, 256);
-  lay->off_own_lse = align_up(lay->off_pre_lse + rows * 4, 256);
-  lay->off_pre_o = align_up(lay->off_own_lse + rows * 4, 256);
-  lay->off_own_o = align_up(lay->off_pre_o + rows * a->own.head_dim * 4, 256);
+  lay->off_own_lse = align_up(lay->off_part + pl->bytes, 256);
+  lay->off_own_o = align_up(lay->off_own_lse + rows * 4, 256);
   lay->bytes = align_up(lay->off_own_o + rows * a->own.head_dim * 4, 256);
   return B2D_OK;
 }
@@ -354,9 +369,7 @@ extern "C" int b2d_cross_attention(const b2d_cross_args* a, void* stream) {
       s.num_tokens = s.num_groups * a->query_len;
     }
     const RaggedParams p = params_of(&s, pl, part);
-    if ((rc = launch_attention(&s, pl, p, st))) return rc;
-    B2D_BY_DIM_AND_TYPE(launch_merge, a->head_dim, a->q_dtype == B2D_BF16, pl, p, st);
-    if (cudaGetLastError() != cudaSuccess) return B2D_ERR_CUDA;
+    if ((rc = launch_both(&s, pl, p, st))) return rc;
   }
   return B2D_OK;
 }
@@ -390,7 +403,8 @@ extern "C" int b2d_decode_shared_prefix(const b2d_shared_prefix_args* a, void* s
   float* own_o = reinterpret_cast<float*>(ws + lay.off_own_o);
   float* own_lse = reinterpret_cast<float*>(ws + lay.off_own_lse);
   // Own tokens first: that call checks the rest of the arguments before it
-  // enqueues anything.  Its part stays in fp32; out is rounded once, by the join.
+  // enqueues anything.  Its part stays in fp32; the prefix kernel joins the two
+  // and rounds once.
   b2d_gqa_args own = a->own;
   own.out = own_o;
   own.out_stride_b = (int64_t)own.num_q_heads * own.head_dim;
@@ -400,9 +414,7 @@ extern "C" int b2d_decode_shared_prefix(const b2d_shared_prefix_args* a, void* s
   own.workspace_bytes = lay.gqa;
   if ((rc = gqa_decode_f32(&own, own_o, stream))) return rc;
   RaggedParams p = params_of(&c, pl, ws + lay.off_part);
-  p.out_f32 = reinterpret_cast<float*>(ws + lay.off_pre_o);
-  p.lse2 = reinterpret_cast<float*>(ws + lay.off_pre_lse);
-  if ((rc = launch_attention(&c, pl, p, st))) return rc;
-  B2D_BY_DIM_AND_TYPE(launch_join, c.head_dim, c.q_dtype == B2D_BF16, pl, p, own_o, own_lse, st);
-  return cudaGetLastError() == cudaSuccess ? B2D_OK : B2D_ERR_CUDA;
+  p.own_o = own_o;
+  p.own_lse = own_lse;
+  return launch_both(&c, pl, p, st);
 }

@@ -60,21 +60,21 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int gq = lane >> 2, tq = lane & 3;
 
+  griddep_wait();
+  griddep_launch();
   ragged_table(p, table, warp_tmp);
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= p.G; i += blockDim.x) p.table_g[i] = table[i];
-  ragged_zero_rows<D, QT>(p);
+  ragged_rows_without_keys<D, QT>(p);
   const int W = table[p.G];
   const int ctas = W < (int)gridDim.x ? W : (int)gridDim.x;
+  if (tid == 0) ragged_note_cut(p, blockIdx.x, nullptr, W, ctas);   // nothing yet
   if ((int)blockIdx.x >= ctas) return;
   const int x0 = range_begin(W, ctas, blockIdx.x), x1 = range_begin(W, ctas, blockIdx.x + 1);
   const uint32_t q32 = smem_u32(sq), k32 = smem_u32(sk), v32 = smem_u32(sv);
   const int mtx = lane >> 3, rr = lane & 7;
 
   int g = find_row(table, p.G, x0);
-  for (int x = x0; x < x1;) {
-    while (x >= table[g + 1]) ++g;
-    const RaggedPiece w = ragged_piece(p, table, g, x, x1);
+  RaggedPiece w;
+  for (int x = x0; ragged_next(p, table, x1, g, x, w);) {
     const int t0 = w.t0 + w.first(0, p.TS), nrows = min(p.TS, w.n - w.first(0, p.TS)) * p.grp;
     __syncthreads();
     for (int i = tid; i < C::kRows * (D / 8); i += 128) {
@@ -184,18 +184,31 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
       }
     }
 
-    const bool whole = w.c0 == 0 && w.c1 == w.nch;
-    const int slot = (w.c0 == 0 && x > x0) ? 1 : 0;
+    const bool whole = w.whole();
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       const int row = 16 * warp + gq + 8 * r;
       if (row >= nrows) continue;
-      const float inv = l[r] > 0.f ? vscale / l[r] : l[r];   // no mass at all: 0; NaN stays
-      const float lse2 = m[r] + fast_log2(l[r]);
+      float inv = l[r] > 0.f ? vscale / l[r] : l[r];   // no mass at all: 0; NaN stays
+      float lse2 = m[r] + fast_log2(l[r]);
       const int t = t0 + row / p.grp, h = w.h * p.grp + row % p.grp;
-      if (whole && p.out_f32 == nullptr) {
+      if (whole) {
+        if (p.own_o != nullptr) {   // join with the sequence's own part
+          const int64_t at = (int64_t)t * p.Hq + h;
+          const float2 jw = join_weights(lse2, p.own_lse[at], lse2);
+          inv *= jw.x;
+          if (jw.y != 0.f) {
+            const float* own = p.own_o + at * D + 2 * tq;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+              acc[i][2 * r] = acc[i][2 * r] * inv + own[8 * i] * jw.y;
+              acc[i][2 * r + 1] = acc[i][2 * r + 1] * inv + own[8 * i + 1] * jw.y;
+            }
+            inv = 1.f;
+          }
+        }
         QT* dst = reinterpret_cast<QT*>(p.out) + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 2 * tq;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
@@ -204,17 +217,16 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
         }
         if (p.lse != nullptr && tq == 0) p.lse[(int64_t)t * p.lse_st + h] = lse2 * kLn2;
       } else {
-        const int64_t at = whole ? (int64_t)t * p.Hq + h
-                                 : (int64_t)(2 * blockIdx.x + slot) * p.rows + row;
-        float* dst = (whole ? p.out_f32 : p.seg_o) + at * D + 2 * tq;
+        const int64_t at = (int64_t)w.segment(blockIdx.x) * p.rows + row;
+        float* dst = p.seg_o + at * D + 2 * tq;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
           *reinterpret_cast<float2*>(dst + 8 * i) =
               make_float2(acc[i][2 * r] * inv, acc[i][2 * r + 1] * inv);
-        if (tq == 0) (whole ? p.lse2 : p.seg_lse)[at] = lse2;
+        if (tq == 0) p.seg_lse[at] = lse2;
       }
     }
-    x += w.c1 - w.c0;
+    if (tid == 0 && w.c0 == 0 && !whole) ragged_note_cut(p, blockIdx.x, &w, W, ctas);
   }
 }
 

@@ -181,18 +181,19 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
     prefetch_tmap(&tmap_v);
   }
   tc_fence_before();
+  griddep_wait();                            // (everything above overlaps the kernel before)
+  griddep_launch();
   ragged_table(p, table, table + p.G + 1);   // ends with __syncthreads
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= p.G; i += blockDim.x) p.table_g[i] = table[i];
-  ragged_zero_rows<D, QT>(p);
+  ragged_rows_without_keys<D, QT>(p);
   const int W = table[p.G];
   const int ctas = W < (int)gridDim.x ? W : (int)gridDim.x;
   const bool active = (int)blockIdx.x < ctas;
   const int x0 = active ? range_begin(W, ctas, blockIdx.x) : 0;
   const int x1 = active ? range_begin(W, ctas, blockIdx.x + 1) : 0;
   const int g_first = active ? find_row(table, p.G, x0) : 0;
+  if (threadIdx.x == 0) ragged_note_cut(p, blockIdx.x, nullptr, W, ctas);   // nothing yet
   // All lanes of a warp see the same answer: one that ran out of time stops all.
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     for (int i = 0; i < 64; ++i)   // the clock is read only after some polls
@@ -264,11 +265,10 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
     int g = g_first;
     bool ok = true;
     RaggedPiece w;
-    if (x0 < x1) {
-      w = ragged_piece(p, table, g, x0, x1);
-      load_q(w);
-    }
-    for (int x = x0; x < x1 && ok;) {
+    int x = x0;
+    bool more = ragged_next(p, table, x1, g, x, w);
+    if (more) load_q(w);
+    while (more) {
       const bool mine = st < w.parts();
       const int nrows = mine ? rows_of(w) : 0;
       const bool live = r0 < nrows;              // this warp has query rows
@@ -335,22 +335,30 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
         }
         l += sum.x + sum.y;
       };
-      // The usual step: no masked key, and no maximum that has to move.
-      // False: nothing was done.
-      auto fast_step = [&]() -> bool {
+      // The usual step: the first of a piece, which sets the maximum, or one that
+      // leaves it.  False: nothing was done.
+      auto fast_step = [&](bool first, int nvalid) -> bool {
         uint32_t v[CH];
 #pragma unroll
         for (int c = 0; c < CH; c += 32) tmem_ld32(t_s + (uint32_t)c, v + c);
         tmem_wait_ld();
-        float mc[4] = {m, m, m, m};
+        if (nvalid < CH) {
+          if (sl == 0.f) return false;           // (a score of -inf times 0 is no weight of 0)
+#pragma unroll
+          for (int j = 0; j < CH; ++j)
+            if (j >= nvalid) v[j] = 0xff800000u;
+        }
+        float mc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int j = 0; j < CH; j += 8)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             mc[k] = max3_nan(mc[k], __uint_as_float(v[j + 2 * k]), __uint_as_float(v[j + 2 * k + 1]));
-        const float cm = max3_nan(mc[0], mc[1], max3_nan(mc[2], mc[3], m));
-        // (a NaN, or infinities on either side, fail this too)
-        if (!__all_sync(0xffffffffu, (cm - m) * sl <= kLazy)) return false;
+        const float cm = max3_nan(mc[0], mc[1], max3_nan(mc[2], mc[3], -INFINITY));
+        const float mn = first ? cm : m;
+        // (a NaN, an infinite maximum, or +inf against a finite one fail this)
+        if (!__all_sync(0xffffffffu, (cm - mn) * sl <= kLazy && fabsf(mn) < INFINITY)) return false;
+        m = mn;
         const float off = -m * sl;
         float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
@@ -369,7 +377,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
         ++ns_all;
         tc_fence_after();
         if (live) {
-          if (i == 0 || nvalid < CH || !fast_step()) full_step(i, nvalid);
+          if (!fast_step(i == 0, nvalid)) full_step(i, nvalid);
           tmem_wait_st();
         }                                        // (rows that do not exist: P is never used)
         tc_fence_before();
@@ -378,14 +386,9 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       if (!ok) break;
       // Q of the next piece, so that its first product runs beside the output.
       const RaggedPiece d = w;
-      const bool whole = d.c0 == 0 && d.c1 == d.nch;
-      const int slot = (d.c0 == 0 && x > x0) ? 1 : 0;
-      x += d.c1 - d.c0;
-      if (x < x1) {
-        while (x >= table[g + 1]) ++g;
-        w = ragged_piece(p, table, g, x, x1);
-        load_q(w);
-      }
+      const bool whole = d.whole();
+      more = ragged_next(p, table, x1, g, x, w);
+      if (more) load_q(w);
       if (!mine) continue;
       if (!wait(o_full + st, outs & 1u)) { ok = false; break; }
       ++outs;
@@ -393,74 +396,93 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       if (live) {
         float vscale = 1.f;
         if constexpr (F8) vscale = p.v_scale ? __ldg(p.v_scale + d.head(st)) : 1.f;
-        const float inv = l > 0.f ? vscale / l : l;
-        const float lse2 = l == 0.f ? -INFINITY : m * sl + fast_log2(l);
-        const bool direct = whole && p.out_f32 == nullptr;
+        float inv = l > 0.f ? vscale / l : l;
+        float lse2 = l == 0.f ? -INFINITY : m * sl + fast_log2(l);
         const int tok = d.t0 + d.first(st, p.TS) + tq, head = d.head(st) * p.grp + hq;
-        const int64_t at = whole ? (int64_t)tok * p.Hq + head
-                                 : (int64_t)(2 * blockIdx.x + slot) * p.rows + st * p.TS * p.grp + r;
-        uint32_t v[D];
-#pragma unroll
-        for (int c = 0; c < D; c += 32) tmem_ld32(t_o + (uint32_t)c, v + c);
-        tmem_wait_ld();
-        tc_fence_before();
-#pragma unroll
-        for (int j = 0; j < D; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * inv);
-        // Through shared memory, 64 bytes of each row at a time, so that a
+        const bool join = whole && p.own_o != nullptr;
+        float own = 0.f;                         // weight of the sequence's own part
+        if (join && r < nrows) {
+          const float2 jw = join_weights(lse2, p.own_lse[(int64_t)tok * p.Hq + head], lse2);
+          inv *= jw.x;
+          own = jw.y;
+        }
+        // Through shared memory, 16 fp32 columns of each row at a time, so that a
         // warp stores whole sectors; 16-byte pieces are permuted by the row
-        // against bank conflicts.
-        const int64_t row_at = direct ? ((int64_t)tok * p.o_st + (int64_t)head * p.o_sh) * 2 : at * (D * 4);
-        uint8_t* gout = direct ? static_cast<uint8_t*>(p.out)
-                               : reinterpret_cast<uint8_t*>(whole ? p.out_f32 : p.seg_o);
-        int64_t dst[4];
+        // against bank conflicts.  Lane k copies piece k % 4 of rows 8i + k / 4.
+        // (Rolled and with few registers: it must not cost the softmax any.)
+        const int64_t at = whole ? (int64_t)tok * p.o_st + (int64_t)head * p.o_sh
+                                 : (int64_t)d.segment(blockIdx.x) * p.rows + st * p.TS * p.grp + r;
+        const int64_t my_row = (int64_t)tok * p.Hq + head;
+        const int piece = lane & 3, row4 = lane >> 2;
+        auto piece_at = [&](int row, int q) { return stage + (uint32_t)(row * 64 + ((q ^ ((row >> 1) & 3)) << 4)); };
+        uint32_t v[16];
+        float4 z[4];                             // own parts of the next columns
+        auto load_own = [&](int c) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          dst[i] = __shfl_sync(0xffffffffu, row_at, 8 * i + (lane >> 2)) + 16 * (lane & 3);
-        auto piece_at = [&](int row, int c) { return stage + (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4)); };
-        auto copy_rows = [&](int shift) {
+          for (int i = 0; i < 4; ++i) {
+            const float ow = __shfl_sync(0xffffffffu, own, 8 * i + row4);
+            const int64_t orow = __shfl_sync(0xffffffffu, my_row, 8 * i + row4);
+            z[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (ow != 0.f) {
+              z[i] = *reinterpret_cast<const float4*>(p.own_o + orow * D + c + 4 * piece);
+              z[i].x *= ow;
+              z[i].y *= ow;
+              z[i].z *= ow;
+              z[i].w *= ow;
+            }
+          }
+        };
+        tmem_ld16(t_o, v);
+        if (join) load_own(0);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+          tmem_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[4 * q + e]) * inv;
+            sts128(piece_at(lane, q), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
+                                                 __float_as_uint(f[2]), __float_as_uint(f[3])));
+          }
+          if (c + 16 < D) tmem_ld16(t_o + (uint32_t)(c + 16), v);
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int rl = 8 * i + (lane >> 2);
-            const uint4 y = lds128(piece_at(rl, lane & 3));
-            if (r0 + rl < nrows) *reinterpret_cast<uint4*>(gout + dst[i] + shift) = y;
-          }
-          __syncwarp();
-        };
-        if (direct) {
-#pragma unroll
-          for (int c = 0; c < D; c += 32) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t o[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                o[e] = pack2<std::is_same<QT, __nv_bfloat16>::value>(
-                    __uint_as_float(v[c + 8 * q + 2 * e]), __uint_as_float(v[c + 8 * q + 2 * e + 1]));
-              sts128(piece_at(lane, q), make_uint4(o[0], o[1], o[2], o[3]));
+            const int rl = 8 * i + row4, cc = c + 4 * piece;
+            uint4 y = lds128(piece_at(rl, piece));
+            const int64_t dst = __shfl_sync(0xffffffffu, at, rl);
+            if (join) {
+              y.x = __float_as_uint(__uint_as_float(y.x) + z[i].x);
+              y.y = __float_as_uint(__uint_as_float(y.y) + z[i].y);
+              y.z = __float_as_uint(__uint_as_float(y.z) + z[i].z);
+              y.w = __float_as_uint(__uint_as_float(y.w) + z[i].w);
             }
-            copy_rows(2 * c);
+            if (r0 + rl < nrows) {
+              if (whole)
+                *reinterpret_cast<uint2*>(reinterpret_cast<QT*>(p.out) + dst + cc) =
+                    make_uint2(pack_pair<QT>(__uint_as_float(y.x), __uint_as_float(y.y)),
+                               pack_pair<QT>(__uint_as_float(y.z), __uint_as_float(y.w)));
+              else
+                *reinterpret_cast<uint4*>(p.seg_o + dst * D + cc) = y;
+            }
           }
-        } else {
-#pragma unroll
-          for (int c = 0; c < D; c += 16) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              sts128(piece_at(lane, q), make_uint4(v[c + 4 * q], v[c + 4 * q + 1], v[c + 4 * q + 2], v[c + 4 * q + 3]));
-            copy_rows(4 * c);
-          }
+          if (join && c + 16 < D) load_own(c + 16);
+          __syncwarp();
         }
+        tc_fence_before();
         if (r < nrows) {
-          if (!direct) (whole ? p.lse2 : p.seg_lse)[at] = lse2;
+          if (!whole) p.seg_lse[at] = lse2;
           else if (p.lse != nullptr) p.lse[(int64_t)tok * p.lse_st + head] = lse2 * kLn2;
         }
       }
+      if (threadIdx.x == 0 && d.c0 == 0 && !whole) ragged_note_cut(p, blockIdx.x, &d, W, ctas);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegOther));
   }
-  // The ring holds, for each chunk of a piece and each KV head of its item, K
-  // and then V: `heads` pairs of slots per chunk.
+  // The ring holds, for each chunk of a piece, K of each KV head of its item
+  // and then V of each: a K slot is free again long before its V is.
   if (warp == 8) {
     // ---------------- MMAs (one thread) ----------------
     if (lane == 0) {
@@ -475,14 +497,12 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
       int g = g_first;
       bool ok = true;
-      for (int x = x0; x < x1 && ok;) {
-        while (x >= table[g + 1]) ++g;
-        const RaggedPiece w = ragged_piece(p, table, g, x, x1);
+      RaggedPiece w;
+      for (int x = x0; ok && ragged_next(p, table, x1, g, x, w);) {
         const int nc = w.c1 - w.c0, parts = w.parts();
-        x += nc;
-        // Ring position of stream st's K of chunk i; whether the stream is the
-        // tile's last reader.
-        auto k_at = [&](int st, int i) { return ring + (uint32_t)(2 * (w.heads * i + (w.heads == 2 ? st : 0))); };
+        // Ring position of stream st's K (its V: `heads` further) of chunk i;
+        // whether the stream is the tile's last reader.
+        auto k_at = [&](int st, int i) { return ring + (uint32_t)(2 * w.heads * i + (w.heads == 2 ? st : 0)); };
         auto last = [&](int st) { return w.heads == 2 || st == parts - 1; };
         auto qk = [&](int st, int i) -> bool {   // S of step i
           const uint32_t n = k_at(st, i), slot = n % NS;
@@ -500,7 +520,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           return true;
         };
         auto pv = [&](int st, int i) -> bool {   // O += P.V of step i
-          const uint32_t n = k_at(st, i) + 1u, slot = n % NS;
+          const uint32_t n = k_at(st, i) + (uint32_t)w.heads, slot = n % NS;
           if (!wait1(full + slot, (n / NS) & 1u) || !wait1(p_full + st, np[st]++ & 1u)) return false;
           tc_fence_after();
           const uint32_t ts = tmem + (uint32_t)(st * 128), to = tmem + 256u + (uint32_t)(st * D);
@@ -538,9 +558,8 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       uint32_t n = 0;
       int g = g_first;
       bool ok = true;
-      for (int x = x0; x < x1 && ok;) {
-        while (x >= table[g + 1]) ++g;
-        const RaggedPiece w = ragged_piece(p, table, g, x, x1);
+      RaggedPiece w;
+      for (int x = x0; ok && ragged_next(p, table, x1, g, x, w);) {
         const int32_t* row = p.block_table + (int64_t)w.g * p.bt_stride;
         auto page_of = [&](int c) -> int {
           const int t = c * CH + gr * granule;
@@ -557,19 +576,19 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           const int left = min(CH, w.len - c * CH);
           const uint32_t tx = (uint32_t)((left + granule - 1) / granule * granule) * kBox * PB;
           const int next = page_of(c + 1);
-          for (int u = 0; u < 2 * w.heads; ++u, ++n) {   // K, V of each head
+          for (int u = 0; u < 2 * w.heads; ++u, ++n) {   // K of each head, V of each head
             const uint32_t slot = n % N;
+            const bool is_v = u >= w.heads;
             if (!wait(eb + slot, ((n / N) & 1u) ^ 1u)) { ok = false; break; }
-            uint64_t* bar = !F8 && (u & 1) && left < CH ? tail + slot : fb + slot;
+            uint64_t* bar = !F8 && is_v && left < CH ? tail + slot : fb + slot;
             if (lane == 0) mbar_arrive_expect_tx(bar, tx);
             __syncwarp();
             if (load)
               tma_load_4d(smem + base + slot * bytes + (uint32_t)(blk * 16384 + gr * granule * (int)kBox),
-                          (u & 1) ? &tmap_v : &tmap_k, bar, blk * 64, t % p.P, w.h + (u >> 1), page, policy);
+                          is_v ? &tmap_v : &tmap_k, bar, blk * 64, t % p.P, w.h + (is_v ? u - w.heads : u), page, policy);
           }
           page = next;
         }
-        x += w.c1 - w.c0;
       }
       // Copies still in flight land before the block ends.
       for (uint32_t i = n > (uint32_t)N ? n - N : 0; i < n; ++i)
@@ -581,17 +600,15 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       uint32_t ring = 0, seen = 0;               // seen: bit s = parity of tail[s]
       int g = g_first;
       bool ok = true;
-      for (int x = x0; x < x1 && ok;) {
-        while (x >= table[g + 1]) ++g;
-        const RaggedPiece w = ragged_piece(p, table, g, x, x1);
+      RaggedPiece w;
+      for (int x = x0; ok && ragged_next(p, table, x1, g, x, w);) {
         const int nc = w.c1 - w.c0;
         const int nvalid = w.len - (w.c1 - 1) * CH;
-        x += nc;
         ring += (uint32_t)(2 * w.heads * nc);
         if (nvalid >= CH) continue;
         const int per = (CH - nvalid) * 8;       // 16-byte pieces of a column block
         for (int h = w.heads; h > 0 && ok; --h) {
-          const uint32_t slot = (ring - 2u * (uint32_t)h + 1u) % NS;
+          const uint32_t slot = (ring - (uint32_t)h) % NS;
           if (!(ok = wait(tail + slot, (seen >> slot) & 1u))) break;
           seen ^= 1u << slot;
           for (int i = lane; i < per * C::kBlk; i += 32) {
@@ -613,9 +630,8 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
     uint32_t n = 0;
     int g = g_first;
     bool ok = true;
-    for (int x = x0; x < x1 && ok;) {
-      while (x >= table[g + 1]) ++g;
-      const RaggedPiece w = ragged_piece(p, table, g, x, x1);
+    RaggedPiece w;
+    for (int x = x0; ok && ragged_next(p, table, x1, g, x, w);) {
       for (int ch = w.c0; ch < w.c1 && ok; ++ch) {
         const int nvalid = min(CH, w.len - ch * CH);
         for (int u = 0; u < 2 * w.heads; ++u, ++n) {
@@ -647,7 +663,6 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           if (lane == 0) mbar_arrive(full + slot);
         }
       }
-      x += w.c1 - w.c0;
     }
   }
   tc_fence_before();

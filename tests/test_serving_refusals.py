@@ -86,8 +86,8 @@ def test_shared_sizes_refused(kw, code):
 def test_shared_calls_refused():
     lib, n = _lib.load(), C.c_size_t(0)
     assert lib.b2d_shared_prefix_workspace_bytes(C.byref(shared_args()), C.byref(n)) == 0
-    # partials of the own tokens and of the prefix: two fp32 copies of out at least
-    assert n.value > 2 * 8 * 32 * 128 * 4
+    # the own tokens' part: one fp32 copy of out at least
+    assert n.value > 8 * 32 * 128 * 4
     call = lambda **kw: lib.b2d_decode_shared_prefix(C.byref(shared_args(**kw)), None)  # noqa: E731
     assert lib.b2d_decode_shared_prefix(None, None) == -1
     assert call() == -1 and call(batch=0) == 0

@@ -16,8 +16,8 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from . import _lib
-from .api import DecodeWorkspace, _check, _ptr
-from .ragged import _ints, _one_device, _workspace
+from .api import B2DError, DecodeWorkspace, _ptr
+from .ragged import _ints, _on, _one_device, _stream, _table, _workspace
 
 
 class AppendPlan(NamedTuple):
@@ -31,27 +31,25 @@ def _pool(where: str, cache_seqlens, block_table, free_pages, free_count, page_s
     if not cache_seqlens.is_cuda:
         raise RuntimeError(f"b200decode.{where} needs CUDA tensors (there is no CPU path)")
     bsz = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else -1
-    _ints(where, (bsz,), cache_seqlens=cache_seqlens)
-    _ints(where, (1,), free_count=free_count)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != bsz:
-        raise ValueError(f"{where}: block_table must be int32 [{bsz}, max_pages]")
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
-        raise ValueError(f"{where}: block_table rows must be contiguous")
+    _ints(where, "cache_seqlens", cache_seqlens, bsz)
+    _ints(where, "free_count", free_count, 1)
+    _table(where, "block_table", block_table, bsz)
     if bsz > 1 and block_table.stride(0) < block_table.shape[1]:
         raise ValueError(f"{where}: block_table rows overlap")
-    if free_pages.dtype != torch.int32 or free_pages.dim() != 1 or not free_pages.is_contiguous():
+    if free_pages.dim() != 1:
         raise ValueError(f"{where}: free_pages must be contiguous int32 [capacity]")
-    if int(page_size) <= 0:
+    _ints(where, "free_pages", free_pages, free_pages.shape[0])
+    if page_size <= 0:
         raise ValueError(f"{where}: page_size must be positive")
     return bsz
 
 
-def _out(where: str, name: str, t: Optional[torch.Tensor], shape: tuple, dtype, device) -> torch.Tensor:
-    if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
-        raise ValueError(f"{where}: {name} must be contiguous {dtype} {list(shape)}")
-    return t
+def _check_out(where: str, name: str, t: torch.Tensor, n: int, dtype: torch.dtype) -> None:
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{where}: {name} must be contiguous {dtype} [{n}]")
+
+
+_HEADER = _lib.B2D_WORKSPACE_HEADER_BYTES
 
 
 def plan_append(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -81,12 +79,11 @@ def plan_append(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pag
     """
     where = "plan_append"
     bsz = _pool(where, cache_seqlens, block_table, free_pages, free_count, page_size)
-    dev = cache_seqlens.device
-    _one_device(where, dev, block_table=block_table, free_pages=free_pages, free_count=free_count,
-                new_tokens=new_tokens, slot_mapping=slot_mapping, query_starts=query_starts,
-                seqlens_out=seqlens_out, free_count_out=free_count_out)
+    index = cache_seqlens.get_device()
+    _one_device(where, index, block_table, free_pages, free_count, new_tokens, slot_mapping, query_starts,
+                seqlens_out, free_count_out)
     if new_tokens is not None:
-        _ints(where, (bsz,), new_tokens=new_tokens)
+        _ints(where, "new_tokens", new_tokens, bsz)
     if max_tokens is None:
         if slot_mapping is not None:
             max_tokens = slot_mapping.shape[0]
@@ -94,23 +91,32 @@ def plan_append(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pag
             max_tokens = bsz
         else:
             raise ValueError(f"{where}: new_tokens needs max_tokens or slot_mapping")
-    with torch.cuda.device(dev):
-        slot_mapping = _out(where, "slot_mapping", slot_mapping, (int(max_tokens),), torch.int64, dev)
-        query_starts = _out(where, "query_starts", query_starts, (bsz + 1,), torch.int32, dev)
-        seqlens_out = _out(where, "seqlens_out", seqlens_out, (bsz,), torch.int32, dev)
-        free_count_out = _out(where, "free_count_out", free_count_out, (1,), torch.int32, dev)
-        a = _lib.PlanAppendArgs()
-        a.cache_seqlens, a.new_tokens = cache_seqlens.data_ptr(), _ptr(new_tokens)
-        a.block_table, a.block_table_stride = block_table.data_ptr(), block_table.stride(0)
-        a.free_pages, a.free_count = free_pages.data_ptr(), free_count.data_ptr()
-        a.slot_mapping, a.query_starts = slot_mapping.data_ptr(), query_starts.data_ptr()
-        a.seqlens_out, a.free_count_out = seqlens_out.data_ptr(), free_count_out.data_ptr()
-        a.num_requests, a.max_pages_per_seq = bsz, block_table.shape[1]
-        a.page_size, a.max_tokens, a.free_capacity = int(page_size), int(max_tokens), free_pages.shape[0]
-        ws = _workspace(workspace, dev, _lib.B2D_WORKSPACE_HEADER_BYTES)
-        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
-        _check(_lib.load().b2d_plan_append(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
-               "b2d_plan_append")
+    if slot_mapping is None:
+        slot_mapping = cache_seqlens.new_empty((max_tokens,), dtype=torch.int64)
+    else:
+        _check_out(where, "slot_mapping", slot_mapping, max_tokens, torch.int64)
+    if query_starts is None:
+        query_starts = cache_seqlens.new_empty((bsz + 1,))
+    else:
+        _check_out(where, "query_starts", query_starts, bsz + 1, torch.int32)
+    if seqlens_out is None:
+        seqlens_out = torch.empty_like(cache_seqlens)
+    else:
+        _check_out(where, "seqlens_out", seqlens_out, bsz, torch.int32)
+    if free_count_out is None:
+        free_count_out = torch.empty_like(free_count)
+    else:
+        _check_out(where, "free_count_out", free_count_out, 1, torch.int32)
+    with _on(index):
+        ws = _workspace(workspace, index, lambda: _HEADER)
+        a = _lib.PlanAppendArgs(cache_seqlens.data_ptr(), _ptr(new_tokens), block_table.data_ptr(),
+                                block_table.stride(0), free_pages.data_ptr(), free_count.data_ptr(),
+                                slot_mapping.data_ptr(), query_starts.data_ptr(), seqlens_out.data_ptr(),
+                                free_count_out.data_ptr(), bsz, block_table.shape[1], page_size, max_tokens,
+                                free_pages.shape[0], 0, ws.ptr, ws.nbytes)
+        rc = _lib.load().b2d_plan_append(C.byref(a), _stream(index))
+    if rc:
+        raise B2DError(rc, "b2d_plan_append")
     return AppendPlan(slot_mapping, query_starts, seqlens_out, free_count_out)
 
 
@@ -129,23 +135,25 @@ def release_pages(cache_seqlens: torch.Tensor, block_table: torch.Tensor, finish
     B2D_ERR_DEVICE_CAPACITY."""
     where = "release_pages"
     bsz = _pool(where, cache_seqlens, block_table, free_pages, free_count, page_size)
-    dev = cache_seqlens.device
-    if finished.dtype != torch.bool or tuple(finished.shape) != (bsz,) or not finished.is_contiguous():
+    if finished.dtype is not torch.bool or finished.shape != (bsz,) or not finished.is_contiguous():
         raise ValueError(f"{where}: finished must be contiguous bool [{bsz}]")
-    _one_device(where, dev, block_table=block_table, finished=finished, free_pages=free_pages,
-                free_count=free_count, seqlens_out=seqlens_out, free_count_out=free_count_out)
-    with torch.cuda.device(dev):
-        seqlens_out = _out(where, "seqlens_out", seqlens_out, (bsz,), torch.int32, dev)
-        free_count_out = _out(where, "free_count_out", free_count_out, (1,), torch.int32, dev)
-        a = _lib.ReleaseArgs()
-        a.cache_seqlens, a.finished = cache_seqlens.data_ptr(), finished.data_ptr()
-        a.block_table, a.block_table_stride = block_table.data_ptr(), block_table.stride(0)
-        a.free_pages, a.free_count = free_pages.data_ptr(), free_count.data_ptr()
-        a.seqlens_out, a.free_count_out = seqlens_out.data_ptr(), free_count_out.data_ptr()
-        a.num_requests, a.max_pages_per_seq = bsz, block_table.shape[1]
-        a.page_size, a.free_capacity = int(page_size), free_pages.shape[0]
-        ws = _workspace(workspace, dev, _lib.B2D_WORKSPACE_HEADER_BYTES)
-        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
-        _check(_lib.load().b2d_release_pages(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
-               "b2d_release_pages")
+    index = cache_seqlens.get_device()
+    _one_device(where, index, block_table, finished, free_pages, free_count, seqlens_out, free_count_out)
+    if seqlens_out is None:
+        seqlens_out = torch.empty_like(cache_seqlens)
+    else:
+        _check_out(where, "seqlens_out", seqlens_out, bsz, torch.int32)
+    if free_count_out is None:
+        free_count_out = torch.empty_like(free_count)
+    else:
+        _check_out(where, "free_count_out", free_count_out, 1, torch.int32)
+    with _on(index):
+        ws = _workspace(workspace, index, lambda: _HEADER)
+        a = _lib.ReleaseArgs(cache_seqlens.data_ptr(), finished.data_ptr(), block_table.data_ptr(),
+                             block_table.stride(0), free_pages.data_ptr(), free_count.data_ptr(),
+                             seqlens_out.data_ptr(), free_count_out.data_ptr(), bsz, block_table.shape[1],
+                             page_size, free_pages.shape[0], ws.ptr, ws.nbytes)
+        rc = _lib.load().b2d_release_pages(C.byref(a), _stream(index))
+    if rc:
+        raise B2DError(rc, "b2d_release_pages")
     return seqlens_out, free_count_out

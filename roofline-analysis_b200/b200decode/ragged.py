@@ -10,49 +10,87 @@ cute_attention/cluster_decode/cluster_decode_reduce.py:67-91.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
-from typing import Optional, Tuple
+from typing import Callable, Optional, Tuple
 
 import torch
 
 from . import _lib
-from .api import _DT, DecodeWorkspace, _check, _default_ws, _gqa_args, _layout_strides, _ptr, decode
+from .api import (_DT, B2DError, DecodeWorkspace, _check, _default_ws, _gqa_args, _layout_strides, _ptr, _ws,
+                  decode)
 
 
-def _one_device(where: str, device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{where}: {name} is on {t.device}, q on {device}")
+_stream = torch._C._cuda_getCurrentRawStream   # of a device index, without a Stream object
+_here = contextlib.nullcontext()
 
 
-def _ints(where: str, shape: tuple, **tensors) -> None:
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or tuple(t.shape) != shape:
-            raise ValueError(f"{where}: {name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-        if not t.is_contiguous():
-            raise ValueError(f"{where}: {name} must be contiguous")
+def _on(index: int):
+    """Makes device `index` the current one (nothing to do, as a rule)."""
+    return _here if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
-def _result(where: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None:
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.stride(-1) != 1:
+def _one_device(where: str, index: int, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{where}: all tensors must be on cuda:{index}, one is on {t.device}")
+
+
+def _ints(where: str, name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{where}: {name} must be contiguous int32 [{n}], got {t.dtype} {list(t.shape)}")
+
+
+def _table(where: str, name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != n or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{where}: {name} must be int32 [{n}, max_pages] with contiguous rows")
+
+
+def _result(where: str, name: str, t: torch.Tensor, shape, dtype: torch.dtype) -> None:
+    if t.shape != shape or t.dtype is not dtype or t.stride(-1) != 1:
         raise ValueError(f"{where}: {name} must be {dtype} {list(shape)} with a contiguous last axis")
 
 
-def _workspace(workspace: Optional[DecodeWorkspace], device: torch.device, need: int) -> DecodeWorkspace:
+def _scales(where: str, hkv: int, k_scale, v_scale) -> None:
+    for s in (k_scale, v_scale):
+        if s is not None and (s.dtype is not torch.float32 or s.numel() != hkv or not s.is_contiguous()):
+            raise ValueError(f"{where}: k_scale and v_scale must be contiguous fp32 with num_kv_heads elements")
+
+
+def _workspace(workspace: Optional[DecodeWorkspace], index: int, need: Callable[[], int]) -> DecodeWorkspace:
     """The caller's workspace, or the default one of the device's current
-    stream.  While that stream is captured into a CUDA graph the default would
-    be shared by every graph captured there, and could be reallocated under
-    them: a call without a workspace of its own then gets one from the graph's
-    memory pool (its header is zeroed by a node of the graph)."""
+    stream (as large as it is: the call says when that is too small).  While
+    that stream is captured into a CUDA graph the default would be shared by
+    every graph captured there, and could be reallocated under them: a call
+    without a workspace of its own then gets one of need() bytes from the
+    graph's memory pool (its header is zeroed by a node of the graph)."""
     capturing = torch.cuda.is_current_stream_capturing()
     if workspace is not None:
-        if workspace.buf.device != device:
-            raise ValueError(f"workspace is on {workspace.buf.device}, the tensors on {device}")
+        if workspace.buf.get_device() != index:
+            raise ValueError(f"workspace is on {workspace.buf.device}, the tensors on cuda:{index}")
         workspace.captured = workspace.captured or capturing
-        return workspace.ensure(need)
+        return workspace.ensure(need()) if capturing else workspace
     if capturing:
-        return DecodeWorkspace.in_graph(device, need)
-    return _default_ws(device).ensure(need)
+        return DecodeWorkspace.in_graph(torch.device("cuda", index), need())
+    return _ws.get((index, _stream(index))) or _default_ws(torch.device("cuda", index))
+
+
+def _call(fn, name: str, a, own, workspace: Optional[DecodeWorkspace], index: int, query) -> None:
+    """fn(a) on the current stream, its workspace (fields of `own`) grown when
+    the library finds it too small (nothing is enqueued before that check)."""
+    def need() -> int:
+        n = C.c_size_t(0)
+        _check(query(C.byref(a), C.byref(n)), name)
+        return n.value
+    ws = _workspace(workspace, index, need)
+    own.workspace, own.workspace_bytes = ws.ptr, ws.nbytes
+    rc = fn(C.byref(a), _stream(index))
+    if rc == _lib.B2D_ERR_WORKSPACE:
+        ws.ensure(need())
+        own.workspace, own.workspace_bytes = ws.ptr, ws.nbytes
+        rc = fn(C.byref(a), _stream(index))
+    if rc:
+        raise B2DError(rc, name)
 
 
 def _cache_fields(a: _lib.CrossArgs, where: str, q: torch.Tensor, k_cache: torch.Tensor,
@@ -119,61 +157,61 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if not q.is_cuda:
         raise RuntimeError("b200decode.cross_attention needs CUDA tensors (there is no CPU path)")
     ragged = query_starts is not None
-    if q.dim() != (3 if ragged else q.dim()) or q.dim() not in (3, 4):
+    dims = q.dim()
+    if dims != 3 and (ragged or dims != 4):
         raise ValueError(f"{where}: q must be [T, Hq, D] with query_starts, or [B, Tq, Hq, D] or [B, Hq, D] "
                          f"without, got {tuple(q.shape)}")
+    index = q.get_device()
+    _one_device(where, index, k_cache, v_cache, kv_lens, block_table, query_starts, k_scale, v_scale, out, lse)
     bsz = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    _ints(where, (bsz,), kv_lens=kv_lens)
-    _one_device(where, q.device, k_cache=k_cache, v_cache=v_cache, kv_lens=kv_lens, block_table=block_table,
-                query_starts=query_starts, k_scale=k_scale, v_scale=v_scale, out=out, lse=lse)
-    if not ragged and q.shape[0] != bsz:
-        raise ValueError(f"{where}: q has {q.shape[0]} requests, kv_lens {bsz}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != bsz:
-        raise ValueError(f"{where}: block_table must be int32 [{bsz}, max_pages]")
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
-        raise ValueError(f"{where}: block_table rows must be contiguous")
+    _ints(where, "kv_lens", kv_lens, bsz)
+    _table(where, "block_table", block_table, bsz)
+    shape = q.shape
+    if not ragged and shape[0] != bsz:
+        raise ValueError(f"{where}: q has {shape[0]} requests, kv_lens {bsz}")
     if q.stride(-1) != 1:
         raise ValueError(f"{where}: the head_dim axis must be contiguous")
-    if softmax_scale is None:
-        softmax_scale = q.shape[-1] ** -0.5
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if lse is None:
-        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
-    _result(where, "out", out, q.shape, q.dtype)
-    _result(where, "lse", lse, q.shape[:-1], torch.float32)
     a = _lib.CrossArgs()
     hkv = _cache_fields(a, where, q, k_cache, v_cache, kv_layout)
-    hq, d = q.shape[-2:]
+    hq, d = shape[-2:]
     if hq % hkv:
         raise ValueError(f"{where}: num_q_heads {hq} must be a multiple of num_kv_heads {hkv}")
-    for s, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if s is not None and (s.dtype != torch.float32 or s.numel() != hkv or not s.is_contiguous()):
-            raise ValueError(f"{where}: {n} must be contiguous fp32 with num_kv_heads elements")
+    if k_scale is not None or v_scale is not None:
+        _scales(where, hkv, k_scale, v_scale)
+    if softmax_scale is None:
+        softmax_scale = d ** -0.5
+    if out is None:
+        out = q.new_empty(shape)
+    else:
+        _result(where, "out", out, shape, q.dtype)
+    if lse is None:
+        lse = q.new_empty(shape[:-1], dtype=torch.float32)
+    else:
+        _result(where, "lse", lse, shape[:-1], torch.float32)
+    q3, out3, lse2, length = q, out, lse, 1
     if ragged:
-        _ints(where, (bsz + 1,), query_starts=query_starts)
-        q3, out3, lse2, length = q, out, lse, 0
-    elif q.dim() == 4:
+        _ints(where, "query_starts", query_starts, bsz + 1)
+        length = 0
+    elif dims == 4:
         # [B, Tq, ...] as [B * Tq, ...]: one token stride
+        length = shape[1]
         q3 = q.reshape(-1, hq, d)
         try:
             out3, lse2 = out.view(-1, hq, d), lse.view(-1, hq)
         except RuntimeError as e:
             raise ValueError(f"{where}: out and lse need one stride for all tokens") from e
-        length = q.shape[1]
-    else:
-        q3, out3, lse2, length = q, out, lse, 1
     if q3.shape[0] == 0 or bsz == 0:
         return out, lse
-    with torch.cuda.device(q.device):
+    lib = _lib.load()
+    with _on(index):
         if length == 1 and not flags:
             ws = workspace
             if ws is not None or torch.cuda.is_current_stream_capturing():
                 g = _gqa_args(q3, k_cache, v_cache, kv_lens, block_table, softmax_scale, k_scale, v_scale, out3,
                               lse2, kv_layout, num_ctas)
                 need = C.c_size_t(0)
-                _check(_lib.load().b2d_gqa_workspace_bytes(C.byref(g), C.byref(need)), "b2d_gqa_workspace_bytes")
-                ws = _workspace(workspace, q.device, need.value)
+                _check(lib.b2d_gqa_workspace_bytes(C.byref(g), C.byref(need)), "b2d_gqa_workspace_bytes")
+                ws = _workspace(workspace, index, lambda: need.value)
             decode(q3, k_cache, v_cache, kv_lens, block_table, softmax_scale, k_scale=k_scale, v_scale=v_scale,
                    out=out3, lse=lse2, kv_layout=kv_layout, num_ctas=num_ctas, workspace=ws,
                    wait_limit_us=wait_limit_us)
@@ -181,22 +219,16 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         a.q, a.q_stride_t, a.q_stride_h = q3.data_ptr(), q3.stride(0), q3.stride(1)
         a.query_starts, a.kv_lens, a.block_table = _ptr(query_starts), kv_lens.data_ptr(), block_table.data_ptr()
         a.block_table_stride = block_table.stride(0)
-        fp8 = k_cache.dtype == torch.float8_e4m3fn
-        a.k_scale, a.v_scale = (_ptr(k_scale), _ptr(v_scale)) if fp8 else (None, None)
+        if k_cache.dtype is torch.float8_e4m3fn:
+            a.k_scale, a.v_scale = _ptr(k_scale), _ptr(v_scale)
         a.out, a.out_stride_t, a.out_stride_h = out3.data_ptr(), out3.stride(0), out3.stride(1)
         a.lse, a.lse_stride_t = lse2.data_ptr(), lse2.stride(0)
         a.num_tokens, a.num_groups, a.query_len = q3.shape[0], bsz, length
         a.num_q_heads, a.head_dim, a.max_pages_per_seq = hq, d, block_table.shape[1]
         a.q_dtype, a.kv_dtype = _DT[q.dtype], _DT[k_cache.dtype]
-        a.softmax_scale, a.num_ctas = float(softmax_scale), int(num_ctas or 0)
-        a.flags, a.wait_limit_us = int(flags), int(wait_limit_us)
-        lib = _lib.load()
-        need = C.c_size_t(0)
-        _check(lib.b2d_cross_workspace_bytes(C.byref(a), C.byref(need)), "b2d_cross_workspace_bytes")
-        ws = _workspace(workspace, q.device, need.value)
-        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
-        _check(lib.b2d_cross_attention(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
-               "b2d_cross_attention")
+        a.softmax_scale, a.num_ctas = softmax_scale, num_ctas or 0
+        a.flags, a.wait_limit_us = flags, wait_limit_us
+        _call(lib.b2d_cross_attention, "b2d_cross_attention", a, a, workspace, index, lib.b2d_cross_workspace_bytes)
     return out, lse
 
 
@@ -234,61 +266,60 @@ def decode_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     where = "decode_shared_prefix"
     if not q.is_cuda:
         raise RuntimeError("b200decode.decode_shared_prefix needs CUDA tensors (there is no CPU path)")
-    _one_device(where, q.device, k_cache=k_cache, v_cache=v_cache, prefix_lens=prefix_lens,
-                prefix_block_table=prefix_block_table, cache_seqlens=cache_seqlens, block_table=block_table,
-                group_starts=group_starts, k_scale=k_scale, v_scale=v_scale, out=out, lse=lse)
+    index = q.get_device()
+    _one_device(where, index, k_cache, v_cache, prefix_lens, prefix_block_table, cache_seqlens, block_table,
+                group_starts, k_scale, v_scale, out, lse)
     groups = prefix_lens.shape[0] if prefix_lens.dim() == 1 else -1
-    _ints(where, (groups,), prefix_lens=prefix_lens)
+    _ints(where, "prefix_lens", prefix_lens, groups)
+    _table(where, "prefix_block_table", prefix_block_table, groups)
     if group_starts is not None:
-        _ints(where, (groups + 1,), group_starts=group_starts)
+        _ints(where, "group_starts", group_starts, groups + 1)
     elif groups > 1:
         raise ValueError(f"{where}: {groups} prefixes need group_starts")
-    if (prefix_block_table.dtype != torch.int32 or prefix_block_table.dim() != 2
-            or prefix_block_table.shape[0] != groups):
-        raise ValueError(f"{where}: prefix_block_table must be int32 [{groups}, max_pages]")
-    if prefix_block_table.stride(1) != 1 and prefix_block_table.shape[1] > 1:
-        raise ValueError(f"{where}: prefix_block_table rows must be contiguous")
     q3 = q[:, 0] if q.dim() == 4 else q
     if q3.dim() != 3:
         raise ValueError(f"{where}: q must be [B, Hq, D] or [B, 1, Hq, D], got {tuple(q.shape)}")
-    if not cache_seqlens.is_contiguous():
-        raise ValueError(f"{where}: cache_seqlens must be contiguous")
-    for s, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if s is not None and not s.is_contiguous():
-            raise ValueError(f"{where}: {n} must be contiguous")
+    shape = q3.shape
+    _ints(where, "cache_seqlens", cache_seqlens, shape[0])
+    if k_scale is not None or v_scale is not None:
+        for s in (k_scale, v_scale):
+            if s is not None and not s.is_contiguous():
+                raise ValueError(f"{where}: k_scale and v_scale must be contiguous")
     if softmax_scale is None:
-        softmax_scale = q3.shape[-1] ** -0.5
+        softmax_scale = shape[-1] ** -0.5
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
+    else:
+        _result(where, "out", out, q.shape, q.dtype)
     if lse is None:
-        lse = torch.empty(q3.shape[:2], dtype=torch.float32, device=q.device)
-    _result(where, "out", out, q.shape, q.dtype)
-    _result(where, "lse", lse, q3.shape[:2], torch.float32)
-    out3 = out[:, 0] if out.dim() == 4 else out
-    with torch.cuda.device(q.device):
-        a = _lib.SharedPrefixArgs()
-        a.own = _gqa_args(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, k_scale, v_scale,
-                          out3, lse, kv_layout, num_ctas)
-        a.own.flags, a.own.wait_limit_us = int(flags), int(wait_limit_us)
-        a.prefix_lens, a.prefix_block_table = prefix_lens.data_ptr(), prefix_block_table.data_ptr()
-        a.prefix_block_table_stride = prefix_block_table.stride(0)
-        a.group_starts = _ptr(group_starts)
-        a.num_groups, a.prefix_max_pages = groups, prefix_block_table.shape[1]
-        lib = _lib.load()
-        need = C.c_size_t(0)
-        _check(lib.b2d_shared_prefix_workspace_bytes(C.byref(a), C.byref(need)),
-               "b2d_shared_prefix_workspace_bytes")
-        ws = _workspace(workspace, q.device, need.value)
-        a.own.workspace, a.own.workspace_bytes = ws.ptr, ws.nbytes
-        _check(lib.b2d_decode_shared_prefix(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
-               "b2d_decode_shared_prefix")
+        lse = q.new_empty(shape[:2], dtype=torch.float32)
+    else:
+        _result(where, "lse", lse, shape[:2], torch.float32)
+    a = _lib.SharedPrefixArgs()
+    a.own = _gqa_args(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, k_scale, v_scale,
+                      out[:, 0] if out.dim() == 4 else out, lse, kv_layout, num_ctas)
+    own = a.own
+    own.flags, own.wait_limit_us = flags, wait_limit_us
+    a.prefix_lens, a.prefix_block_table = prefix_lens.data_ptr(), prefix_block_table.data_ptr()
+    a.prefix_block_table_stride = prefix_block_table.stride(0)
+    a.group_starts = _ptr(group_starts)
+    a.num_groups, a.prefix_max_pages = groups, prefix_block_table.shape[1]
+    lib = _lib.load()
+    with _on(index):
+        _call(lib.b2d_decode_shared_prefix, "b2d_decode_shared_prefix", a, own, workspace, index,
+              lib.b2d_shared_prefix_workspace_bytes)
     return out, lse
+
+
+_MERGE = {torch.bfloat16: _lib.B2D_BF16, torch.float16: _lib.B2D_FP16, torch.float32: _lib.B2D_FP32}
 
 
 def _span(t: torch.Tensor) -> Tuple[int, int]:
     """First and last byte address + 1 that a (non-empty) tensor covers."""
-    first = t.data_ptr()
-    return first, first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    first, elems = t.data_ptr(), 1
+    for n, s in zip(t.shape, t.stride()):
+        elems += (n - 1) * s
+    return first, first + elems * t.element_size()
 
 
 def merge_states(outs: torch.Tensor, lses: torch.Tensor, *, out: Optional[torch.Tensor] = None,
@@ -307,41 +338,40 @@ def merge_states(outs: torch.Tensor, lses: torch.Tensor, *, out: Optional[torch.
     where = "merge_states"
     if not outs.is_cuda:
         raise RuntimeError("b200decode.merge_states needs CUDA tensors (there is no CPU path)")
-    if outs.dim() != 4 or outs.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if outs.dim() != 4 or outs.dtype not in _MERGE:
         raise ValueError(f"{where}: outs must be bf16, fp16 or fp32 [N, T, H, D], got {outs.dtype} {tuple(outs.shape)}")
-    if lses.dtype != torch.float32 or lses.shape != outs.shape[:3]:
-        raise ValueError(f"{where}: lses must be fp32 {list(outs.shape[:3])}")
-    if outs.stride(3) != 1:
+    shape = outs.shape
+    if lses.dtype is not torch.float32 or lses.shape != shape[:3]:
+        raise ValueError(f"{where}: lses must be fp32 {list(shape[:3])}")
+    so, sl = outs.stride(), lses.stride()
+    if so[3] != 1:
         raise ValueError(f"{where}: the head_dim axis must be contiguous")
-    _one_device(where, outs.device, lses=lses, out=out, lse=lse)
-    n, t, h, d = outs.shape
+    index = outs.get_device()
+    _one_device(where, index, lses, out, lse)
+    n, t, h, d = shape
+    given = out is not None or lse is not None
     if out is None:
-        out = torch.empty(t, h, d, dtype=outs.dtype, device=outs.device)
+        out = outs.new_empty((t, h, d))
+    else:
+        if (out.dtype is not outs.dtype and outs.dtype is not torch.float32) or out.dtype not in _MERGE:
+            raise ValueError(f"{where}: out must be {outs.dtype} like the states, or 16-bit from fp32 states")
+        _result(where, "out", out, shape[1:], out.dtype)
     if lse is None:
-        lse = torch.empty(t, h, dtype=torch.float32, device=outs.device)
-    if out.dtype != outs.dtype and outs.dtype != torch.float32:
-        raise ValueError(f"{where}: out must be {outs.dtype} like the states")
-    if out.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise ValueError(f"{where}: out must be bf16, fp16 or fp32, got {out.dtype}")
-    _result(where, "out", out, (t, h, d), out.dtype)
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (t, h):
+        lse = lses.new_empty((t, h))
+    elif lse.dtype is not torch.float32 or lse.shape != shape[1:3]:
         raise ValueError(f"{where}: lse must be fp32 [{t}, {h}]")
-    if out.numel():
-        spans = [(_span(x), f"{name}") for x, name in ((outs, "outs"), (lses, "lses"))]
+    if given and out.numel():
+        inputs = (_span(outs), _span(lses))
         for x, name in ((out, "out"), (lse, "lse")):
-            a0, a1 = _span(x)
-            for (b0, b1), other in spans:
-                if a0 < b1 and b0 < a1:
-                    raise ValueError(f"{where}: {name} overlaps {other}")
-    a = _lib.MergeArgs()
-    a.outs, a.outs_stride_n, a.outs_stride_t, a.outs_stride_h = outs.data_ptr(), *outs.stride()[:3]
-    a.lses, a.lses_stride_n, a.lses_stride_t, a.lses_stride_h = lses.data_ptr(), *lses.stride()
-    a.out, a.out_stride_t, a.out_stride_h = out.data_ptr(), *out.stride()[:2]
-    a.lse, a.lse_stride_t, a.lse_stride_h = lse.data_ptr(), *lse.stride()
-    a.num_states, a.num_tokens, a.num_heads, a.head_dim = n, t, h, d
-    dt = {**_DT, torch.float32: _lib.B2D_FP32}
-    a.in_dtype, a.out_dtype = dt[outs.dtype], dt[out.dtype]
-    with torch.cuda.device(outs.device):
-        _check(_lib.load().b2d_merge_states(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
-               "b2d_merge_states")
+            first, end = _span(x)
+            if any(first < e and f < end for f, e in inputs):
+                raise ValueError(f"{where}: {name} overlaps an input")
+    wo, wl = out.stride(), lse.stride()
+    a = _lib.MergeArgs(outs.data_ptr(), so[0], so[1], so[2], lses.data_ptr(), sl[0], sl[1], sl[2],
+                       out.data_ptr(), wo[0], wo[1], lse.data_ptr(), wl[0], wl[1],
+                       n, t, h, d, _MERGE[outs.dtype], _MERGE[out.dtype])
+    with _on(index):
+        rc = _lib.load().b2d_merge_states(C.byref(a), _stream(index))
+    if rc:
+        raise B2DError(rc, "b2d_merge_states")
     return out, lse

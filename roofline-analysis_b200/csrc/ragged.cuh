@@ -34,7 +34,7 @@
 
 namespace b2d {
 
-constexpr int kItemCost = 1;   // positions of an item on the line before its first chunk
+constexpr int kItemCost = 3;   // positions of an item on the line before its first chunk
 
 struct RaggedParams {
   const void* q;

@@ -563,7 +563,10 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
         const int32_t* row = p.block_table + (int64_t)w.g * p.bt_stride;
         auto page_of = [&](int c) -> int {
           const int t = c * CH + gr * granule;
-          return gr < granules && c < w.c1 && t < w.len ? __ldg(row + t / p.P) : 0;
+          int pg = 0;   // (volatile: loaded a chunk ahead of its use, not at it)
+          if (gr < granules && c < w.c1 && t < w.len)
+            asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(pg) : "l"(row + t / p.P));
+          return pg;
         };
         int page = page_of(w.c0);
         for (int c = w.c0; c < w.c1 && ok; ++c) {

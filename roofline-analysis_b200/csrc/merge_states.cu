@@ -4,11 +4,13 @@
 // lse = M + ln sum w_i.
 //
 // HBM-bound: every state is read once, the result written once.  A thread
-// owns 8 consecutive elements of a row (16-byte loads; two for fp32) and
-// loops over the states, U = 4 of them loaded before any is used.  It computes
-// the row's weights itself, from N broadcast loads: cheaper than a barrier.
-// A state with lse = -inf is skipped, not multiplied by 0, so it may hold
-// anything.
+// owns 8 consecutive elements of a row (16-byte loads; two for fp32) and takes
+// the states U at a time: their values and lse are loaded together, one round
+// trip to memory, and folded in with a running maximum.  It computes the
+// row's weights itself, from broadcast loads: cheaper than a barrier.  A state
+// with lse = -inf is left out, not multiplied by 0, so it may hold anything.
+// 8 bf16 states of [256, 32, 128], 19 MB: 6.8 us, 2.8 TB/s, of which about 3 us
+// are launch and one round trip.
 #include <type_traits>
 
 #include "b2d_decode.h"
@@ -30,16 +32,30 @@ struct MergeParams {
   int64_t work;  // rows * D / 8
 };
 
+// 8 elements as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* src, float* v) {
-  if constexpr (std::is_same<T, float>::value) {
-    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+struct Raw8 {
+  uint4 w;
+  __device__ __forceinline__ void get(float* v) const {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 f;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) f = bf16x2_to_f2(x[i]);
+      else f = f16x2_to_f2(x[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+template <>
+struct __align__(16) Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void get(float* v) const {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    load_q8<T>(src, v);
   }
-}
+};
 
 template <typename T>
 __device__ __forceinline__ void store8(T* dst, const float* v) {
@@ -54,7 +70,7 @@ __device__ __forceinline__ void store8(T* dst, const float* v) {
 template <typename IT, typename OT>
 __global__ void __launch_bounds__(256) merge_states_kernel(const MergeParams p) {
   constexpr float kLog2e = 1.4426950408889634f;
-  constexpr int U = 4;
+  constexpr int U = std::is_same<IT, float>::value ? 4 : 8;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= p.work) return;
   const int64_t row = i / p.D8;
@@ -64,34 +80,40 @@ __global__ void __launch_bounds__(256) merge_states_kernel(const MergeParams p) 
   const float* ls = p.lses + t * p.lt + (int64_t)h * p.lh;
   const IT* src = reinterpret_cast<const IT*>(p.outs) + t * p.st + (int64_t)h * p.sh + c;
   float mx = -INFINITY;
-  for (int n = 0; n < p.N; ++n) mx = fmaxf(mx, ls[n * p.ln]);
-  const float mz = mx == -INFINITY ? 0.f : mx;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
   for (int n0 = 0; n0 < p.N; n0 += U) {
-    float v[U][8], l[U];
+    Raw8<IT> raw[U];
+    float l[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      l[u] = n0 + u < p.N ? ls[(n0 + u) * p.ln] : -INFINITY;
-      if (l[u] != -INFINITY) {
-        load8<IT>(src + (n0 + u) * p.sn, v[u]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
-      }
+      const int n = n0 + u < p.N ? n0 + u : p.N - 1;
+      raw[u] = *reinterpret_cast<const Raw8<IT>*>(src + n * p.sn);
+      l[u] = n0 + u < p.N ? ls[n * p.ln] : -INFINITY;
     }
+    float nm = mx;
+#pragma unroll
+    for (int u = 0; u < U; ++u) nm = fmaxf(nm, l[u]);
+    const float mz = nm == -INFINITY ? 0.f : nm, old = fast_exp2((mx - mz) * kLog2e);
+    sum *= old;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= old;
+    mx = nm;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (l[u] == -INFINITY) continue;
       const float w = fast_exp2((l[u] - mz) * kLog2e);
+      float v[8];
+      raw[u].get(v);
       sum += w;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += w * v[u][e];
+      for (int e = 0; e < 8; ++e) acc[e] += w * v[e];
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] *= inv;
   store8<OT>(reinterpret_cast<OT*>(p.out) + t * p.ot + (int64_t)h * p.oh + c, acc);
-  if (p.lse != nullptr && c == 0) p.lse[t * p.let + (int64_t)h * p.leh] = mz + logf(sum);
+  if (p.lse != nullptr && c == 0) p.lse[t * p.let + (int64_t)h * p.leh] = mx == -INFINITY ? mx + sum : mx + logf(sum);
 }
 
 }  // namespace b2d

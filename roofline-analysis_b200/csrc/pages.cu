@@ -13,8 +13,9 @@
 // from L2, the sums stay in shared memory) and then does its share of the
 // slots and table entries, finding each one's request by bisection; no block
 // waits for another.  The lengths and the free count may be updated in
-// place: the block that is last to finish reading (an arrival counter in the
-// workspace header, zero between calls) writes them.
+// place: then the block that is last to finish reading (an arrival counter in
+// the workspace header, zero between calls) writes them.  A thread takes 4
+// slots at a time, so that their table reads are in flight together.
 #include "b2d_decode.h"
 #include "common.cuh"
 #include "host_common.h"
@@ -39,6 +40,7 @@ struct PagesParams {
   int* status;
   int* arrivals;
   int B, max_pages, P, max_tokens, capacity;
+  int in_place;                 // an output is an input: written by the last block
 };
 
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, int P) { return (tokens + P - 1) / P; }
@@ -117,60 +119,71 @@ __device__ __forceinline__ bool last_block(int* arrivals) {
 
 __global__ void __launch_bounds__(kPageThreads) plan_append_kernel(const PagesParams p) {
   extern __shared__ int32_t sm[];
-  int32_t* tok_start = sm;          // [B]
-  int32_t* page_start = sm + p.B;   // [B]
+  int32_t* tok_start = sm;             // [B]
+  int32_t* page_start = sm + p.B;      // [B]
+  int32_t* lens = sm + 2 * p.B;        // [B]
   const int tid = threadIdx.x;
+  const int count_in = *p.free_count;
   const int per = (p.B + kPageThreads - 1) / kPageThreads;
   const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
   int64_t toks = 0, pages = 0;
   bool fits = true;
   for (int b = b0; b < b1; ++b) {
     const int64_t L = length_of(p, b), n = new_of(p, b);
-    const int64_t end = pages_of(L + n, p.P);
+    const int64_t end = pages_of(L + n, p.P), need = end - pages_of(L, p.P);
+    lens[b] = (int)L;
+    tok_start[b] = (int)n;             // counts, for now
+    page_start[b] = need > INT32_MAX ? INT32_MAX : (int)need;
     toks += n;
-    pages += end - pages_of(L, p.P);
+    pages += need;
     fits = fits && (n == 0 || end <= p.max_pages);
   }
   int64_t total_toks, total_pages;
   block_scan2(toks, pages, total_toks, total_pages);
-  const int count_in = *p.free_count;
   const int count = max(0, min(count_in, p.capacity));
   fits = __syncthreads_and(fits && total_toks <= p.max_tokens && total_pages <= count);
-  for (int b = b0; b < b1; ++b) {   // used only when the totals fit 32 bits
+  for (int b = b0; b < b1; ++b) {   // sums that are used only when the totals fit 32 bits
+    const int n = tok_start[b], need = page_start[b];
     tok_start[b] = (int)toks;
     page_start[b] = (int)pages;
-    const int64_t L = length_of(p, b), n = new_of(p, b);
     toks += n;
-    pages += pages_of(L + n, p.P) - pages_of(L, p.P);
+    pages += need;
   }
   __syncthreads();
   const int first = blockIdx.x * kPageThreads + tid, step = gridDim.x * kPageThreads;
   for (int b = first; b <= p.B; b += step)
     p.starts[b] = !fits ? 0 : (b == p.B ? (int)total_toks : tok_start[b]);
   const int nt = fits ? (int)total_toks : 0, np = fits ? (int)total_pages : 0;
-  for (int t = first; t < p.max_tokens; t += step) {
-    int64_t slot = -1;
-    if (t < nt) {
-      const int b = request_of(tok_start, p.B, t);
-      const int L = length_of(p, b), have = (int)pages_of(L, p.P);
-      const int pos = L + (t - tok_start[b]), pi = pos / p.P;
-      const int page = pi < have ? p.table[b * p.table_stride + pi]
-                                 : p.free_pages[count - 1 - (page_start[b] + pi - have)];
-      if (page >= 0) slot = (int64_t)page * p.P + (pos - pi * p.P);
+  constexpr int U = 4;
+  for (int t0 = first; t0 < p.max_tokens; t0 += U * step) {
+    int page[U], off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * step;
+      page[u] = -1;
+      off[u] = 0;
+      if (t < nt) {
+        const int b = request_of(tok_start, p.B, t);
+        const int L = lens[b], have = (int)pages_of(L, p.P);
+        const int pos = L + (t - tok_start[b]), pi = pos / p.P;
+        page[u] = pi < have ? p.table[b * p.table_stride + pi]
+                            : p.free_pages[count - 1 - (page_start[b] + pi - have)];
+        off[u] = pos - pi * p.P;
+      }
     }
-    p.slots[t] = slot;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * step;
+      if (t < p.max_tokens) p.slots[t] = page[u] < 0 ? -1 : (int64_t)page[u] * p.P + off[u];
+    }
   }
   for (int k = first; k < np; k += step) {
     const int b = request_of(page_start, p.B, k);
-    const int have = (int)pages_of(length_of(p, b), p.P);
+    const int have = (int)pages_of(lens[b], p.P);
     p.table[b * p.table_stride + have + (k - page_start[b])] = p.free_pages[count - 1 - k];
   }
-  if (!last_block(p.arrivals)) return;
-  for (int b = tid; b < p.B; b += kPageThreads) {
-    const int n = new_of(p, b);
-    const int L = p.lens[b];
-    p.lens_out[b] = fits ? (L < 0 ? 0 : L) + n : L;
-  }
+  if (p.in_place ? !last_block(p.arrivals) : blockIdx.x != 0) return;
+  for (int b = tid; b < p.B; b += kPageThreads) p.lens_out[b] = fits ? lens[b] + new_of(p, b) : p.lens[b];
   if (tid == 0) {
     *p.count_out = fits ? count - np : count_in;
     if (!fits) record_status(p.status, kStatusCapacity);
@@ -181,6 +194,7 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const Pages
   extern __shared__ int32_t sm[];
   int32_t* page_start = sm;   // [B]
   const int tid = threadIdx.x;
+  const int count_in = *p.free_count;
   const int per = (p.B + kPageThreads - 1) / kPageThreads;
   const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
   auto given = [&](int b) -> int64_t {
@@ -191,7 +205,6 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const Pages
   int64_t pages = 0, unused = 0, total, unused_total;
   for (int b = b0; b < b1; ++b) pages += given(b);
   block_scan2(pages, unused, total, unused_total);
-  const int count_in = *p.free_count;
   const int count = max(0, min(count_in, p.capacity));
   const bool fits = total <= p.capacity - count;
   for (int b = b0; b < b1; ++b) {   // used only when the total fits 32 bits
@@ -204,7 +217,7 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const Pages
     const int b = request_of(page_start, p.B, k);
     p.free_pages[count + k] = p.table[b * p.table_stride + (k - page_start[b])];
   }
-  if (!last_block(p.arrivals)) return;
+  if (p.in_place ? !last_block(p.arrivals) : blockIdx.x != 0) return;
   for (int b = tid; b < p.B; b += kPageThreads) {
     const int L = p.lens[b];
     p.lens_out[b] = fits && p.finished[b] ? 0 : L;
@@ -234,7 +247,7 @@ extern "C" int b2d_plan_append(const b2d_plan_append_args* a, void* stream) {
   if (!a || a->num_requests < 0 || a->max_pages_per_seq <= 0 || a->page_size <= 0 ||
       a->max_tokens < 0 || a->free_capacity < 0)
     return B2D_ERR_INVALID_ARG;
-  if (a->num_requests > kMaxRequests ||
+  if (a->num_requests > kMaxRequests || a->max_tokens > (1 << 30) ||
       (int64_t)a->max_pages_per_seq * a->page_size > (int64_t)INT32_MAX)
     return B2D_ERR_TOO_LARGE;
   if ((a->num_requests > 0 && (!a->cache_seqlens || !a->block_table || !a->seqlens_out)) ||
@@ -260,9 +273,16 @@ extern "C" int b2d_plan_append(const b2d_plan_append_args* a, void* stream) {
   p.P = a->page_size;
   p.max_tokens = a->max_tokens;
   p.capacity = a->free_capacity;
+  // Any output array that starts inside an input one counts as that one.
+  auto inside = [](const void* out, const void* in, size_t n) {
+    return (uintptr_t)out + n > (uintptr_t)in && (uintptr_t)in + n > (uintptr_t)out;
+  };
+  const size_t rows = (size_t)p.B * 4;
+  p.in_place = inside(p.lens_out, p.lens, rows) || inside(p.count_out, p.free_count, 4) ||
+               (p.new_tokens && inside(p.lens_out, p.new_tokens, rows));
   int sms = 0;
   if (device_sm_count(&sms)) return B2D_ERR_CUDA;
-  const size_t smem = (size_t)p.B * 8;
+  const size_t smem = (size_t)p.B * 12;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(plan_append_kernel), smem)) return B2D_ERR_CUDA;
   plan_append_kernel<<<page_blocks(p.max_tokens, sms), kPageThreads, smem,
                        static_cast<cudaStream_t>(stream)>>>(p);
@@ -296,6 +316,13 @@ extern "C" int b2d_release_pages(const b2d_release_args* a, void* stream) {
   p.max_pages = a->max_pages_per_seq;
   p.P = a->page_size;
   p.capacity = a->free_capacity;
+  // Any output array that starts inside an input one counts as that one.
+  auto inside = [](const void* out, const void* in, size_t n) {
+    return (uintptr_t)out + n > (uintptr_t)in && (uintptr_t)in + n > (uintptr_t)out;
+  };
+  const size_t rows = (size_t)p.B * 4;
+  p.in_place = inside(p.lens_out, p.lens, rows) || inside(p.count_out, p.free_count, 4) ||
+               (p.new_tokens && inside(p.lens_out, p.new_tokens, rows));
   int sms = 0;
   if (device_sm_count(&sms)) return B2D_ERR_CUDA;
   const size_t smem = (size_t)p.B * 4;

@@ -234,28 +234,31 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       const uint32_t flip = scale_of(w) < 0.f ? 0x80008000u : 0u;
       const int64_t mine = (int64_t)(w.t0 + w.first(st, p.TS) + tq) * p.q_st +
                            (int64_t)(w.head(st) * p.grp + hq) * p.q_sh;
-      uint4 v[kCpr];
+#pragma unroll 1
+      for (int i0 = 0; i0 < kCpr; i0 += 8) {
+        uint4 v[8];
 #pragma unroll
-      for (int i = 0; i < kCpr; ++i) {
-        const int rl = i * kRpi + lane / kCpr;
-        const int64_t at = __shfl_sync(0xffffffffu, mine, rl);
-        v[i] = make_uint4(0, 0, 0, 0);
-        if (r0 + rl < nrows)
-          v[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const QT*>(p.q) + at + 8 * (lane % kCpr));
-      }
-#pragma unroll
-      for (int i = 0; i < kCpr; ++i) {
-        const int rl = i * kRpi + lane / kCpr, c = lane % kCpr;
-        if constexpr (F8 && std::is_same<QT, __nv_bfloat16>::value) {
-          uint32_t* e = reinterpret_cast<uint32_t*>(&v[i]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = bf16x2_to_f2(e[j]);
-            e[j] = pack2<false>(f.x, f.y);
-          }
+        for (int i = 0; i < 8; ++i) {
+          const int rl = (i0 + i) * kRpi + lane / kCpr;
+          const int64_t at = __shfl_sync(0xffffffffu, mine, rl);
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (r0 + rl < nrows)
+            v[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const QT*>(p.q) + at + 8 * (lane % kCpr));
         }
-        v[i].x ^= flip; v[i].y ^= flip; v[i].z ^= flip; v[i].w ^= flip;
-        sts128(swz(q_base + (uint32_t)(c >> 3) * 16384u, r0 + rl, c & 7), v[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rl = (i0 + i) * kRpi + lane / kCpr, c = lane % kCpr;
+          if constexpr (F8 && std::is_same<QT, __nv_bfloat16>::value) {
+            uint32_t* e = reinterpret_cast<uint32_t*>(&v[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = bf16x2_to_f2(e[j]);
+              e[j] = pack2<false>(f.x, f.y);
+            }
+          }
+          v[i].x ^= flip; v[i].y ^= flip; v[i].z ^= flip; v[i].w ^= flip;
+          sts128(swz(q_base + (uint32_t)(c >> 3) * 16384u, r0 + rl, c & 7), v[i]);
+        }
       }
       fence_async_smem();
       arrive(q_full + st);
@@ -264,17 +267,114 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
     uint32_t ns_all = 0, outs = 0;               // steps and outputs so far
     int g = g_first;
     bool ok = true;
-    RaggedPiece w;
-    int x = x0;
-    bool more = ragged_next(p, table, x1, g, x, w);
-    if (more) load_q(w);
-    while (more) {
-      const bool mine = st < w.parts();
-      const int nrows = mine ? rows_of(w) : 0;
-      const bool live = r0 < nrows;              // this warp has query rows
-      const float sl = fabsf(scale_of(w));
+    RaggedPiece w, d;                            // the next piece and the one before it
+    int x = x0, nrows = 0;
+    bool mine = false, live = false;             // d has this part; this warp has rows of it
+    float sl = 0.f, m = 0.f, l = 0.f;
+    for (;;) {
+      // Q of the next piece first, so that its first product runs beside the
+      // output of the last.
+      const bool more = ragged_next(p, table, x1, g, x, w);
+      if (more) load_q(w);
+      if (mine) {
+        const bool whole = d.whole();
+        if (!wait(o_full + st, outs & 1u)) { ok = false; break; }
+        ++outs;
+        tc_fence_after();
+        if (live) {
+          float vscale = 1.f;
+          if constexpr (F8) vscale = p.v_scale ? __ldg(p.v_scale + d.head(st)) : 1.f;
+          float inv = l > 0.f ? vscale / l : l;
+          float lse2 = l == 0.f ? -INFINITY : m * sl + fast_log2(l);
+          const int tok = d.t0 + d.first(st, p.TS) + tq, head = d.head(st) * p.grp + hq;
+          const bool join = whole && p.own_o != nullptr;
+          float own = 0.f;                         // weight of the sequence's own part
+          if (join && r < nrows) {
+            const float2 jw = join_weights(lse2, p.own_lse[(int64_t)tok * p.Hq + head], lse2);
+            inv *= jw.x;
+            own = jw.y;
+          }
+          // Through shared memory, 16 fp32 columns of each row at a time, so that a
+          // warp stores whole sectors; 16-byte pieces are permuted by the row
+          // against bank conflicts.  Lane k copies piece k % 4 of rows 8i + k / 4.
+          // (Rolled and with few registers: it must not cost the softmax any.)
+          const int64_t at = whole ? (int64_t)tok * p.o_st + (int64_t)head * p.o_sh
+                                   : (int64_t)d.segment(blockIdx.x) * p.rows + st * p.TS * p.grp + r;
+          const int64_t my_row = (int64_t)tok * p.Hq + head;
+          const int piece = lane & 3, row4 = lane >> 2;
+          auto piece_at = [&](int row, int q) { return stage + (uint32_t)(row * 64 + ((q ^ ((row >> 1) & 3)) << 4)); };
+          uint32_t v[16];
+          float4 z[4];                             // own parts of the next columns
+          auto load_own = [&](int c) {
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float ow = __shfl_sync(0xffffffffu, own, 8 * i + row4);
+              const int64_t orow = __shfl_sync(0xffffffffu, my_row, 8 * i + row4);
+              z[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (ow != 0.f) {
+                z[i] = *reinterpret_cast<const float4*>(p.own_o + orow * D + c + 4 * piece);
+                z[i].x *= ow;
+                z[i].y *= ow;
+                z[i].z *= ow;
+                z[i].w *= ow;
+              }
+            }
+          };
+          tmem_ld16(t_o, v);
+          if (join) load_own(0);
+  #pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            tmem_wait_ld();
+  #pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float f[4];
+  #pragma unroll
+              for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[4 * q + e]) * inv;
+              sts128(piece_at(lane, q), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
+                                                   __float_as_uint(f[2]), __float_as_uint(f[3])));
+            }
+            if (c + 16 < D) tmem_ld16(t_o + (uint32_t)(c + 16), v);
+            __syncwarp();
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rl = 8 * i + row4, cc = c + 4 * piece;
+              uint4 y = lds128(piece_at(rl, piece));
+              const int64_t dst = __shfl_sync(0xffffffffu, at, rl);
+              if (join) {
+                y.x = __float_as_uint(__uint_as_float(y.x) + z[i].x);
+                y.y = __float_as_uint(__uint_as_float(y.y) + z[i].y);
+                y.z = __float_as_uint(__uint_as_float(y.z) + z[i].z);
+                y.w = __float_as_uint(__uint_as_float(y.w) + z[i].w);
+              }
+              if (r0 + rl < nrows) {
+                if (whole)
+                  *reinterpret_cast<uint2*>(reinterpret_cast<QT*>(p.out) + dst + cc) =
+                      make_uint2(pack_pair<QT>(__uint_as_float(y.x), __uint_as_float(y.y)),
+                                 pack_pair<QT>(__uint_as_float(y.z), __uint_as_float(y.w)));
+                else
+                  *reinterpret_cast<uint4*>(p.seg_o + dst * D + cc) = y;
+              }
+            }
+            if (join && c + 16 < D) load_own(c + 16);
+            __syncwarp();
+          }
+          tc_fence_before();
+          if (r < nrows) {
+            if (!whole) p.seg_lse[at] = lse2;
+            else if (p.lse != nullptr) p.lse[(int64_t)tok * p.lse_st + head] = lse2 * kLn2;
+          }
+        }
+        if (threadIdx.x == 0 && d.c0 == 0 && !whole) ragged_note_cut(p, blockIdx.x, &d, W, ctas);
+      }
+      if (!more) break;
+      d = w;
+      mine = st < d.parts();
+      nrows = mine ? rows_of(d) : 0;
+      live = r0 < nrows;
+      sl = fabsf(scale_of(d));
+      m = -INFINITY;
+      l = 0.f;
       const float2 sl2 = make_float2(sl, sl);
-      float m = -INFINITY, l = 0.f;
       // P of 32 scores with offset off, and their sum; with a limit, P is 0 from
       // that score on.
       auto weights = [&](const uint32_t* v, float off, uint32_t* pk, float2& sum, int limit = 32) {
@@ -370,9 +470,9 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
         l += (s0.x + s0.y) + (s1.x + s1.y);
         return true;
       };
-      const int steps = mine ? w.c1 - w.c0 : 0;
+      const int steps = mine ? d.c1 - d.c0 : 0;
       for (int i = 0; i < steps; ++i) {
-        const int nvalid = min(CH, w.len - (w.c0 + i) * CH);
+        const int nvalid = min(CH, d.len - (d.c0 + i) * CH);
         if (!wait(s_full + st, ns_all & 1u)) { ok = false; break; }
         ++ns_all;
         tc_fence_after();
@@ -384,99 +484,6 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
         arrive(p_full + st);
       }
       if (!ok) break;
-      // Q of the next piece, so that its first product runs beside the output.
-      const RaggedPiece d = w;
-      const bool whole = d.whole();
-      more = ragged_next(p, table, x1, g, x, w);
-      if (more) load_q(w);
-      if (!mine) continue;
-      if (!wait(o_full + st, outs & 1u)) { ok = false; break; }
-      ++outs;
-      tc_fence_after();
-      if (live) {
-        float vscale = 1.f;
-        if constexpr (F8) vscale = p.v_scale ? __ldg(p.v_scale + d.head(st)) : 1.f;
-        float inv = l > 0.f ? vscale / l : l;
-        float lse2 = l == 0.f ? -INFINITY : m * sl + fast_log2(l);
-        const int tok = d.t0 + d.first(st, p.TS) + tq, head = d.head(st) * p.grp + hq;
-        const bool join = whole && p.own_o != nullptr;
-        float own = 0.f;                         // weight of the sequence's own part
-        if (join && r < nrows) {
-          const float2 jw = join_weights(lse2, p.own_lse[(int64_t)tok * p.Hq + head], lse2);
-          inv *= jw.x;
-          own = jw.y;
-        }
-        // Through shared memory, 16 fp32 columns of each row at a time, so that a
-        // warp stores whole sectors; 16-byte pieces are permuted by the row
-        // against bank conflicts.  Lane k copies piece k % 4 of rows 8i + k / 4.
-        // (Rolled and with few registers: it must not cost the softmax any.)
-        const int64_t at = whole ? (int64_t)tok * p.o_st + (int64_t)head * p.o_sh
-                                 : (int64_t)d.segment(blockIdx.x) * p.rows + st * p.TS * p.grp + r;
-        const int64_t my_row = (int64_t)tok * p.Hq + head;
-        const int piece = lane & 3, row4 = lane >> 2;
-        auto piece_at = [&](int row, int q) { return stage + (uint32_t)(row * 64 + ((q ^ ((row >> 1) & 3)) << 4)); };
-        uint32_t v[16];
-        float4 z[4];                             // own parts of the next columns
-        auto load_own = [&](int c) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float ow = __shfl_sync(0xffffffffu, own, 8 * i + row4);
-            const int64_t orow = __shfl_sync(0xffffffffu, my_row, 8 * i + row4);
-            z[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (ow != 0.f) {
-              z[i] = *reinterpret_cast<const float4*>(p.own_o + orow * D + c + 4 * piece);
-              z[i].x *= ow;
-              z[i].y *= ow;
-              z[i].z *= ow;
-              z[i].w *= ow;
-            }
-          }
-        };
-        tmem_ld16(t_o, v);
-        if (join) load_own(0);
-#pragma unroll 1
-        for (int c = 0; c < D; c += 16) {
-          tmem_wait_ld();
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float f[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[4 * q + e]) * inv;
-            sts128(piece_at(lane, q), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
-                                                 __float_as_uint(f[2]), __float_as_uint(f[3])));
-          }
-          if (c + 16 < D) tmem_ld16(t_o + (uint32_t)(c + 16), v);
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rl = 8 * i + row4, cc = c + 4 * piece;
-            uint4 y = lds128(piece_at(rl, piece));
-            const int64_t dst = __shfl_sync(0xffffffffu, at, rl);
-            if (join) {
-              y.x = __float_as_uint(__uint_as_float(y.x) + z[i].x);
-              y.y = __float_as_uint(__uint_as_float(y.y) + z[i].y);
-              y.z = __float_as_uint(__uint_as_float(y.z) + z[i].z);
-              y.w = __float_as_uint(__uint_as_float(y.w) + z[i].w);
-            }
-            if (r0 + rl < nrows) {
-              if (whole)
-                *reinterpret_cast<uint2*>(reinterpret_cast<QT*>(p.out) + dst + cc) =
-                    make_uint2(pack_pair<QT>(__uint_as_float(y.x), __uint_as_float(y.y)),
-                               pack_pair<QT>(__uint_as_float(y.z), __uint_as_float(y.w)));
-              else
-                *reinterpret_cast<uint4*>(p.seg_o + dst * D + cc) = y;
-            }
-          }
-          if (join && c + 16 < D) load_own(c + 16);
-          __syncwarp();
-        }
-        tc_fence_before();
-        if (r < nrows) {
-          if (!whole) p.seg_lse[at] = lse2;
-          else if (p.lse != nullptr) p.lse[(int64_t)tok * p.lse_st + head] = lse2 * kLn2;
-        }
-      }
-      if (threadIdx.x == 0 && d.c0 == 0 && !whole) ragged_note_cut(p, blockIdx.x, &d, W, ctas);
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegOther));

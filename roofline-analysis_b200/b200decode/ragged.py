@@ -17,8 +17,7 @@ from typing import Callable, Optional, Tuple
 import torch
 
 from . import _lib
-from .api import (_DT, B2DError, DecodeWorkspace, _check, _default_ws, _gqa_args, _layout_strides, _ptr, _ws,
-                  decode)
+from .api import _DT, B2DError, DecodeWorkspace, _check, _default_ws, _gqa_args, _ptr, _ws, decode
 
 
 _stream = torch._C._cuda_getCurrentRawStream   # of a device index, without a Stream object
@@ -32,7 +31,7 @@ def _on(index: int):
 
 def _one_device(where: str, index: int, *tensors) -> None:
     for t in tensors:
-        if t is not None and t.get_device() != index:
+        if t is not None and t.get_device() != index:   # (-1: a CPU tensor)
             raise ValueError(f"{where}: all tensors must be on cuda:{index}, one is on {t.device}")
 
 
@@ -49,6 +48,12 @@ def _table(where: str, name: str, t: torch.Tensor, n: int) -> None:
 def _result(where: str, name: str, t: torch.Tensor, shape, dtype: torch.dtype) -> None:
     if t.shape != shape or t.dtype is not dtype or t.stride(-1) != 1:
         raise ValueError(f"{where}: {name} must be {dtype} {list(shape)} with a contiguous last axis")
+
+
+def _apart(where: str, out: torch.Tensor, q: torch.Tensor) -> None:
+    # (other overlaps are the caller's to avoid; this is the likely one)
+    if out.data_ptr() == q.data_ptr() and out.numel():
+        raise ValueError(f"{where}: out must not be q: its rows are read until the last is written")
 
 
 def _scales(where: str, hkv: int, k_scale, v_scale) -> None:
@@ -83,7 +88,8 @@ def _call(fn, name: str, a, own, workspace: Optional[DecodeWorkspace], index: in
         _check(query(C.byref(a), C.byref(n)), name)
         return n.value
     ws = _workspace(workspace, index, need)
-    own.workspace, own.workspace_bytes = ws.ptr, ws.nbytes
+    buf = ws.buf
+    own.workspace, own.workspace_bytes = buf.data_ptr(), buf.numel()
     rc = fn(C.byref(a), _stream(index))
     if rc == _lib.B2D_ERR_WORKSPACE:
         ws.ensure(need())
@@ -93,38 +99,37 @@ def _call(fn, name: str, a, own, workspace: Optional[DecodeWorkspace], index: in
         raise B2DError(rc, name)
 
 
-def _cache_fields(a: _lib.CrossArgs, where: str, q: torch.Tensor, k_cache: torch.Tensor,
-                  v_cache: torch.Tensor, kv_layout: str) -> int:
-    """Fills the cache fields of `a`; returns the number of KV heads."""
-    if q.dtype not in (torch.bfloat16, torch.float16):
+def _caches(where: str, q: torch.Tensor, d: int, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_layout: str):
+    """Checks the caches; (k strides, v strides, pages, page size, KV heads,
+    layout) for the library, strides as (page, token, head)."""
+    kd = k_cache.dtype
+    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
         raise ValueError(f"{where}: q dtype must be bf16 or fp16, got {q.dtype}")
-    if k_cache.dtype != v_cache.dtype or k_cache.dtype not in (q.dtype, torch.float8_e4m3fn):
-        raise ValueError(f"{where}: cache dtype {k_cache.dtype} must equal q's {q.dtype} or be float8_e4m3fn")
-    d = q.shape[-1]
+    if kd is not v_cache.dtype or (kd is not q.dtype and kd is not torch.float8_e4m3fn):
+        raise ValueError(f"{where}: cache dtype {kd} must equal q's {q.dtype} or be float8_e4m3fn")
+    shape = k_cache.shape
     if kv_layout == "vllm":
-        if k_cache.dim() != 5 or v_cache.dim() != 4 or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        if len(shape) != 5 or v_cache.dim() != 4 or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
             raise ValueError(f"{where}: kv_layout='vllm' takes contiguous K [blocks, Hkv, D/x, P, x] and V "
                              "[blocks, Hkv, D, P]")
-        nb, hkv, dx, page, x = k_cache.shape
-        if x * k_cache.element_size() != 16 or tuple(v_cache.shape) != (nb, hkv, dx * x, page) or dx * x != d:
+        nb, hkv, dx, page, x = shape
+        if x * k_cache.element_size() != 16 or v_cache.shape != (nb, hkv, dx * x, page) or dx * x != d:
             raise ValueError(f"{where}: vLLM cache shapes do not match")
-        ks, vs = (k_cache.stride(0), x, k_cache.stride(1)), (v_cache.stride(0), 1, v_cache.stride(1))
-        a.kv_layout = _lib.B2D_KV_VLLM
-    else:
-        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
-            raise ValueError(f"{where}: k_cache and v_cache must be matching 4-D paged caches")
-        if k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
-            raise ValueError(f"{where}: the head_dim axis must be contiguous")
-        if k_cache.shape[-1] != d:
-            raise ValueError(f"{where}: head_dim mismatch between q and the caches")
-        *ks, page, hkv = _layout_strides(k_cache, kv_layout)
-        *vs, _, _ = _layout_strides(v_cache, kv_layout)
-        a.kv_layout = _lib.B2D_KV_STRIDED
-    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    a.k_stride_page, a.k_stride_tok, a.k_stride_head = ks
-    a.v_stride_page, a.v_stride_tok, a.v_stride_head = vs
-    a.num_pages, a.page_size, a.num_kv_heads = k_cache.shape[0], page, hkv
-    return hkv
+        return ((k_cache.stride(0), x, k_cache.stride(1)), (v_cache.stride(0), 1, v_cache.stride(1)),
+                nb, page, hkv, _lib.B2D_KV_VLLM)
+    if len(shape) != 4 or shape != v_cache.shape:
+        raise ValueError(f"{where}: k_cache and v_cache must be matching 4-D paged caches")
+    nb, page, hkv, dc = shape
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError(f"{where}: the head_dim axis must be contiguous")
+    if dc != d:
+        raise ValueError(f"{where}: head_dim mismatch between q and the caches")
+    if kv_layout == "NHD":
+        return ks[:3], vs[:3], nb, page, hkv, _lib.B2D_KV_STRIDED
+    if kv_layout == "HND":
+        return (ks[0], ks[2], ks[1]), (vs[0], vs[2], vs[1]), nb, hkv, page, _lib.B2D_KV_STRIDED
+    raise ValueError(f"kv_layout must be 'NHD', 'HND' or 'vllm', got {kv_layout!r}")
 
 
 def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -147,7 +152,7 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     block_table int32 [B, max_pages].  softmax_scale defaults to 1/sqrt(D).
     Returns out (shape of q) and lse (shape of q without D, fp32, natural
     log).  A request without states gives out = 0, lse = -inf; ragged tokens
-    behind query_starts[B] are left as they were.
+    behind query_starts[B] are left as they were.  out must not overlap q.
 
     Captured into a CUDA graph without `workspace`, a call keeps its scratch
     in the graph's memory pool; check_device_status() reads the status only of
@@ -171,9 +176,8 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"{where}: q has {shape[0]} requests, kv_lens {bsz}")
     if q.stride(-1) != 1:
         raise ValueError(f"{where}: the head_dim axis must be contiguous")
-    a = _lib.CrossArgs()
-    hkv = _cache_fields(a, where, q, k_cache, v_cache, kv_layout)
     hq, d = shape[-2:]
+    ks, vs, pages, page, hkv, layout = _caches(where, q, d, k_cache, v_cache, kv_layout)
     if hq % hkv:
         raise ValueError(f"{where}: num_q_heads {hq} must be a multiple of num_kv_heads {hkv}")
     if k_scale is not None or v_scale is not None:
@@ -181,9 +185,10 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if softmax_scale is None:
         softmax_scale = d ** -0.5
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _result(where, "out", out, shape, q.dtype)
+        _apart(where, out, q)
     if lse is None:
         lse = q.new_empty(shape[:-1], dtype=torch.float32)
     else:
@@ -204,7 +209,8 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         return out, lse
     lib = _lib.load()
     with _on(index):
-        if length == 1 and not flags:
+        # One token each is decode(); head_dim 192 outside what that is built for stays here.
+        if length == 1 and not flags and (d != 192 or (page % 16 == 0 and k_cache.dtype is q.dtype)):
             ws = workspace
             if ws is not None or torch.cuda.is_current_stream_capturing():
                 g = _gqa_args(q3, k_cache, v_cache, kv_lens, block_table, softmax_scale, k_scale, v_scale, out3,
@@ -216,18 +222,15 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                    out=out3, lse=lse2, kv_layout=kv_layout, num_ctas=num_ctas, workspace=ws,
                    wait_limit_us=wait_limit_us)
             return out, lse
-        a.q, a.q_stride_t, a.q_stride_h = q3.data_ptr(), q3.stride(0), q3.stride(1)
-        a.query_starts, a.kv_lens, a.block_table = _ptr(query_starts), kv_lens.data_ptr(), block_table.data_ptr()
-        a.block_table_stride = block_table.stride(0)
-        if k_cache.dtype is torch.float8_e4m3fn:
-            a.k_scale, a.v_scale = _ptr(k_scale), _ptr(v_scale)
-        a.out, a.out_stride_t, a.out_stride_h = out3.data_ptr(), out3.stride(0), out3.stride(1)
-        a.lse, a.lse_stride_t = lse2.data_ptr(), lse2.stride(0)
-        a.num_tokens, a.num_groups, a.query_len = q3.shape[0], bsz, length
-        a.num_q_heads, a.head_dim, a.max_pages_per_seq = hq, d, block_table.shape[1]
-        a.q_dtype, a.kv_dtype = _DT[q.dtype], _DT[k_cache.dtype]
-        a.softmax_scale, a.num_ctas = softmax_scale, num_ctas or 0
-        a.flags, a.wait_limit_us = flags, wait_limit_us
+        fp8 = k_cache.dtype is torch.float8_e4m3fn
+        qs, so = q3.stride(), out3.stride()
+        a = _lib.CrossArgs(
+            q3.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), *ks, *vs, pages,
+            _ptr(query_starts), kv_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+            _ptr(k_scale) if fp8 else None, _ptr(v_scale) if fp8 else None,
+            out3.data_ptr(), so[0], so[1], lse2.data_ptr(), lse2.stride(0),
+            q3.shape[0], bsz, length, hq, hkv, d, page, block_table.shape[1], _DT[q.dtype], _DT[k_cache.dtype],
+            softmax_scale, None, 0, num_ctas or 0, flags, layout, wait_limit_us)
         _call(lib.b2d_cross_attention, "b2d_cross_attention", a, a, workspace, index, lib.b2d_cross_workspace_bytes)
     return out, lse
 
@@ -253,7 +256,7 @@ def decode_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     holds sequences group_starts[g] .. group_starts[g + 1] - 1 (sequences
     outside every group have no prefix); None: one group with the whole batch.
     The rest as in decode().  Out is computed in fp32 over both parts and
-    rounded once.
+    rounded once; it must not overlap q.
 
     With a table whose rows begin with a common prefix of n full pages, pass
     prefix_block_table = table[:1, :n], block_table = table[:, n:] and the
@@ -281,29 +284,41 @@ def decode_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         raise ValueError(f"{where}: q must be [B, Hq, D] or [B, 1, Hq, D], got {tuple(q.shape)}")
     shape = q3.shape
     _ints(where, "cache_seqlens", cache_seqlens, shape[0])
-    if k_scale is not None or v_scale is not None:
-        for s in (k_scale, v_scale):
-            if s is not None and not s.is_contiguous():
-                raise ValueError(f"{where}: k_scale and v_scale must be contiguous")
+    if q.dim() == 4 and q.shape[1] != 1:
+        raise ValueError(f"{where}: one query token per sequence (q [B, 1, Hq, D]), got {tuple(q.shape)}")
     if softmax_scale is None:
         softmax_scale = shape[-1] ** -0.5
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _result(where, "out", out, q.shape, q.dtype)
+        _apart(where, out, q)
     if lse is None:
         lse = q.new_empty(shape[:2], dtype=torch.float32)
     else:
         _result(where, "lse", lse, shape[:2], torch.float32)
-    a = _lib.SharedPrefixArgs()
-    a.own = _gqa_args(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, k_scale, v_scale,
-                      out[:, 0] if out.dim() == 4 else out, lse, kv_layout, num_ctas)
+    hq, d = shape[1:]
+    ks, vs, pages, page, hkv, layout = _caches(where, q, d, k_cache, v_cache, kv_layout)
+    if hq % hkv:
+        raise ValueError(f"{where}: num_q_heads {hq} must be a multiple of num_kv_heads {hkv}")
+    if q3.stride(2) != 1:
+        raise ValueError(f"{where}: the head_dim axis must be contiguous")
+    if k_scale is not None or v_scale is not None:
+        _scales(where, hkv, k_scale, v_scale)
+    _table(where, "block_table", block_table, shape[0])
+    out3 = out[:, 0] if out.dim() == 4 else out
+    fp8 = k_cache.dtype is torch.float8_e4m3fn
+    qs, so = q3.stride(), out3.stride()
+    a = _lib.SharedPrefixArgs((
+        q3.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), *ks, *vs, pages,
+        cache_seqlens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+        _ptr(k_scale) if fp8 else None, _ptr(v_scale) if fp8 else None,
+        out3.data_ptr(), so[0], so[1], lse.data_ptr(), lse.stride(0),
+        shape[0], hq, hkv, d, page, block_table.shape[1], _DT[q.dtype], _DT[k_cache.dtype],
+        softmax_scale, None, 0, num_ctas or 0, flags, layout, wait_limit_us),
+        prefix_lens.data_ptr(), prefix_block_table.data_ptr(), prefix_block_table.stride(0), _ptr(group_starts),
+        groups, prefix_block_table.shape[1])
     own = a.own
-    own.flags, own.wait_limit_us = flags, wait_limit_us
-    a.prefix_lens, a.prefix_block_table = prefix_lens.data_ptr(), prefix_block_table.data_ptr()
-    a.prefix_block_table_stride = prefix_block_table.stride(0)
-    a.group_starts = _ptr(group_starts)
-    a.num_groups, a.prefix_max_pages = groups, prefix_block_table.shape[1]
     lib = _lib.load()
     with _on(index):
         _call(lib.b2d_decode_shared_prefix, "b2d_decode_shared_prefix", a, own, workspace, index,

@@ -34,8 +34,9 @@ static int check_sizes(const b2d_cross_args* a) {
   if (a->kv_dtype != a->q_dtype && a->kv_dtype != B2D_FP8_E4M3) return B2D_ERR_UNSUPPORTED;
   if (a->num_q_heads / a->num_kv_heads > 32) return B2D_ERR_UNSUPPORTED;
   if (a->page_size > (1 << 24)) return B2D_ERR_TOO_LARGE;
-  if ((int64_t)a->max_pages_per_seq * a->page_size > (int64_t)INT32_MAX) return B2D_ERR_TOO_LARGE;
-  if (a->wait_limit_us < 0) return B2D_ERR_INVALID_ARG;
+  // (a chunk's last position stays a 32-bit number)
+  if ((int64_t)a->max_pages_per_seq * a->page_size > (int64_t)INT32_MAX - 256) return B2D_ERR_TOO_LARGE;
+  if (a->wait_limit_us < 0 || (a->flags & ~B2D_FLAG_TEST_NO_LOADS)) return B2D_ERR_INVALID_ARG;
   if (a->kv_layout != B2D_KV_STRIDED && a->kv_layout != B2D_KV_VLLM) return B2D_ERR_INVALID_ARG;
   if (a->kv_layout == B2D_KV_VLLM && (a->kv_dtype == B2D_FP8_E4M3 || a->page_size % 16 != 0))
     return B2D_ERR_UNSUPPORTED;

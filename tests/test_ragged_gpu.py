@@ -168,6 +168,56 @@ def test_cross_minus_infinity_scores(cuda):
         assert (out[66:] == 0).all() and torch.isneginf(lse[66:]).all()
 
 
+@pytest.mark.parametrize("kv", [BF, HF, F8])
+@pytest.mark.parametrize("num_ctas", [None, 1, 9])
+def test_cross_nan_and_infinity_in_keys(cuda, kv, num_ctas):
+    """A key of NaN (or one whose score is +inf) among a request's keys makes
+    its rows NaN, on its KV head and nowhere else; in a masked place it changes
+    nothing (make() has NaN there)."""
+    lens, tq, d = [500, 300, 200], [40, 9, 70], 128
+    gen, k, v, _, _, bt = make(cuda, 64, lens, 16, 2, d, kv, "NHD", extra_pages=0)
+    q = torch.rand(119, 4, d, generator=gen, device=cuda).add_(0.1).to(BF if kv != HF else HF)
+    st = torch.tensor([0, 40, 49, 119], dtype=torch.int32, device=cuda)
+    kl = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    clean, _ = b200decode.cross_attention(q, k, v, kl, bt, query_starts=st, num_ctas=num_ctas)
+    assert torch.isfinite(clean).all()
+    for pos in (0, 77, 333, 499):
+        bad = k.clone()
+        raw, code = (bad.view(torch.uint8), 0x7F) if kv == F8 else (bad, float("nan") if pos != 77 else float("inf"))
+        raw[bt[0, pos // 16].long(), pos % 16, 1, 5] = code
+        out, lse = b200decode.cross_attention(q, bad, v, kl, bt, query_starts=st, num_ctas=num_ctas)
+        assert torch.isnan(out[:40, 2:]).all() and torch.isnan(lse[:40, 2:]).all(), pos
+        assert torch.equal(out[:40, :2], clean[:40, :2]) and torch.equal(out[40:], clean[40:]), pos
+
+
+def test_cross_fuzz(cuda):
+    """Random shapes of every kind against the reference."""
+    import random
+    rng = random.Random(11)
+    for i in range(60):
+        kv = rng.choice([BF, HF, F8])
+        qd = HF if kv == HF else rng.choice([BF, HF]) if kv == F8 else BF
+        hkv, grp, d = rng.choice([1, 2, 3, 4]), rng.choice([1, 2, 3, 5, 6, 7, 8, 16, 31, 32]), rng.choice([64, 128])
+        P, layout = rng.choice([16, 32, 48, 64, 112, 128, 256]), rng.choice(["NHD", "HND"])
+        B = rng.randint(1, 6)
+        lens = [rng.choice([0, 1, 63, 64, 65, 127, 128, 129, rng.randint(1, 900)]) for _ in range(B)]
+        tq = [rng.choice([0, 1, 2, rng.randint(1, 150)]) for _ in range(B)]
+        gen, k, v, ks, vs, bt = make(cuda, 1000 + i, lens, P, hkv, d, kv, layout)
+        starts = [0]
+        for n in tq:
+            starts.append(starts[-1] + n)
+        if starts[-1] == 0:
+            continue
+        q = torch.randn(starts[-1], hkv * grp, d, generator=gen, device=cuda).to(qd)
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+        out, lse = b200decode.cross_attention(q, k, v, i32(lens), bt, query_starts=i32(starts), k_scale=ks, v_scale=vs,
+                                              kv_layout=layout, num_ctas=rng.choice([None, None, 2, 13, 300]))
+        ref = cross_reference(q, k, v, ks, vs, bt, starts, lens, d ** -0.5, layout)
+        check(out, ref[0], ref[2], u_of(qd), f"{i} out")
+        check_lse(lse, ref[1], ref[3])
+    b200decode.check_device_status()
+
+
 def shared_reference(q, k, v, ks, vs, pbt, plens, bt, lens, starts, scale, layout):
     out = []
     for b in range(q.shape[0]):

@@ -25,7 +25,7 @@ def cross_args(**kw):
     (dict(head_dim=96), -2), (dict(head_dim=0), -2), (dict(num_q_heads=30), -1), (dict(num_kv_heads=0), -1),
     (dict(num_q_heads=8 * 33), -2), (dict(q_dtype=_lib.B2D_FP8_E4M3), -2), (dict(kv_dtype=_lib.B2D_FP16), -2),
     (dict(page_size=0), -1), (dict(max_pages_per_seq=0), -1), (dict(num_tokens=-1), -1), (dict(num_groups=-1), -1),
-    (dict(query_len=-1), -1), (dict(kv_layout=9), -1), (dict(wait_limit_us=-1), -1),
+    (dict(query_len=-1), -1), (dict(kv_layout=9), -1), (dict(wait_limit_us=-1), -1), (dict(flags=1), -1),
     (dict(kv_layout=_lib.B2D_KV_VLLM, kv_dtype=_lib.B2D_FP8_E4M3), -2),
     (dict(kv_layout=_lib.B2D_KV_VLLM, page_size=8), -2),
     (dict(max_pages_per_seq=1 << 28), -8), (dict(page_size=1 << 25), -8),
@@ -128,6 +128,8 @@ def test_pages_refused():
         for k in ("cache_seqlens", "block_table", "free_pages", "free_count", "seqlens_out", "free_count_out",
                   *(x for x in more if x != "max_tokens")):
             assert call(**{k: None}) == -1, k
+        if fn is lib.b2d_plan_append:
+            assert call(max_tokens=(1 << 30) + 1) == -8
         assert call(num_requests=16385) == -8 and call(max_pages_per_seq=1 << 28) == -8
         assert call(workspace=None) == -4 and call(workspace_bytes=100) == -4 and call(workspace=8) == -3
 
@@ -184,6 +186,9 @@ class TestOnGpu:
             q, kc, kl, bt, st = (x[n] for n in ("q", "kc", "kl", "bt", "st"))
         with pytest.raises(ValueError):
             b200decode.cross_attention(q, kc, kc, kl, bt, query_starts=st, **kw)
+        q, kc, kl, bt, st = self.args(cuda)
+        with pytest.raises(ValueError, match="out must not be q"):
+            b200decode.cross_attention(q, kc, kc, kl, bt, query_starts=st, out=q)
 
     def test_shared(self, cuda):
         q, kc, kl, bt, st = self.args(cuda)
@@ -201,6 +206,10 @@ class TestOnGpu:
             call(q, kc, kc, kl[:1], bt[:1].cpu(), kl, bt)
         with pytest.raises(ValueError):
             call(q, kc, kc, kl[:1], bt[:1], kl, bt, out=q.float())
+        with pytest.raises(ValueError, match="out must not be q"):
+            call(q, kc, kc, kl[:1], bt[:1], kl, bt, out=q)
+        with pytest.raises(ValueError, match="one query token"):
+            call(q[None], kc, kc, kl[:1], bt[:1], kl[:1], bt[:1])
 
     def test_merge(self, cuda):
         o, l = torch.zeros(2, 3, 4, 64, device=cuda), torch.zeros(2, 3, 4, device=cuda)

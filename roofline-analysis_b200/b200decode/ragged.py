@@ -332,6 +332,8 @@ _MERGE = {torch.bfloat16: _lib.B2D_BF16, torch.float16: _lib.B2D_FP16, torch.flo
 def _span(t: torch.Tensor) -> Tuple[int, int]:
     """First and last byte address + 1 that a (non-empty) tensor covers."""
     first, elems = t.data_ptr(), 1
+    if t.is_contiguous():
+        return first, first + t.nbytes
     for n, s in zip(t.shape, t.stride()):
         elems += (n - 1) * s
     return first, first + elems * t.element_size()
@@ -376,11 +378,11 @@ def merge_states(outs: torch.Tensor, lses: torch.Tensor, *, out: Optional[torch.
     elif lse.dtype is not torch.float32 or lse.shape != shape[1:3]:
         raise ValueError(f"{where}: lse must be fp32 [{t}, {h}]")
     if given and out.numel():
-        inputs = (_span(outs), _span(lses))
-        for x, name in ((out, "out"), (lse, "lse")):
+        (o0, o1), (l0, l1) = _span(outs), _span(lses)
+        for x in (out, lse):
             first, end = _span(x)
-            if any(first < e and f < end for f, e in inputs):
-                raise ValueError(f"{where}: {name} overlaps an input")
+            if (first < o1 and o0 < end) or (first < l1 and l0 < end):
+                raise ValueError(f"{where}: out or lse overlaps an input")
     wo, wl = out.stride(), lse.stride()
     a = _lib.MergeArgs(outs.data_ptr(), so[0], so[1], so[2], lses.data_ptr(), sl[0], sl[1], sl[2],
                        out.data_ptr(), wo[0], wo[1], lse.data_ptr(), wl[0], wl[1],

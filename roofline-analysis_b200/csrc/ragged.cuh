@@ -94,10 +94,19 @@ __device__ __forceinline__ int ragged_items(const RaggedParams& p, int n) {
   return p.pairs ? p.Hkv * (tiles >> 1) + (tiles & 1) * ((p.Hkv + 1) >> 1) : p.Hkv * tiles;
 }
 
-// table[g] = line positions of all items before group g (block-wide scan; ends with
-// __syncthreads).  warp_tmp: 32 ints.
-__device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* table,
-                                             int32_t* warp_tmp) {
+// The groups in shared memory: table[g] = line positions of all items before
+// group g, [G + 1]; 32 ints of scratch; and, for up to kCachedGroups groups,
+// first token, tokens and keys of each, so that finding a piece waits for no
+// global load.
+constexpr int kCachedGroups = 1024;
+__host__ __device__ constexpr size_t ragged_table_bytes(int groups) {
+  return ((size_t)groups + 1 + 32 + (groups <= kCachedGroups ? 3 * (size_t)groups : 0)) * 4;
+}
+
+// Fills the table (block-wide scan; ends with __syncthreads).
+__device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* table) {
+  int32_t* warp_tmp = table + p.G + 1;
+  int32_t* cache = p.G <= kCachedGroups ? warp_tmp + 32 : nullptr;
   const int tid = threadIdx.x, nth = blockDim.x;
   const int lane = tid & 31, warp = tid >> 5, nwarps = nth >> 5;
   int carry = 0;
@@ -105,8 +114,14 @@ __device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* tab
     const int g = base + tid;
     int n = 0;
     if (g < p.G) {
-      const int nch = (ragged_kv_len(p, g) + p.CH - 1) / p.CH;
-      n = nch > 0 ? ragged_items(p, ragged_tokens(p, g).y) * (nch + kItemCost) : 0;
+      const int2 tok = ragged_tokens(p, g);
+      const int len = ragged_kv_len(p, g), nch = (len + p.CH - 1) / p.CH;
+      n = nch > 0 ? ragged_items(p, tok.y) * (nch + kItemCost) : 0;
+      if (cache != nullptr) {
+        cache[g] = tok.x;
+        cache[p.G + g] = tok.y;
+        cache[2 * p.G + g] = len;
+      }
     }
     int x = n;
 #pragma unroll
@@ -155,12 +170,19 @@ __device__ __forceinline__ bool ragged_next(const RaggedParams& p, const int32_t
   while (x < x1) {
     while (x >= table[g + 1]) ++g;
     w.g = g;
-    const int2 tok = ragged_tokens(p, g);
-    w.t0 = tok.x;
-    w.n = tok.y;
-    w.len = ragged_kv_len(p, g);
+    if (p.G <= kCachedGroups) {
+      const int32_t* cache = table + p.G + 1 + 32 + g;
+      w.t0 = cache[0];
+      w.n = cache[p.G];
+      w.len = cache[2 * p.G];
+    } else {
+      const int2 tok = ragged_tokens(p, g);
+      w.t0 = tok.x;
+      w.n = tok.y;
+      w.len = ragged_kv_len(p, g);
+    }
     w.nch = (w.len + p.CH - 1) / p.CH;
-    const int tiles = (tok.y + p.TS - 1) / p.TS;
+    const int tiles = (w.n + p.TS - 1) / p.TS;
     const int rel = x - table[g], size = w.nch + kItemCost;
     const int it = rel / size, pos = rel - it * size, end = min(size, pos + (x1 - x));
     w.c0 = max(0, pos - kItemCost);

@@ -80,7 +80,7 @@ static int make_plan(const b2d_cross_args* a, RaggedPlan* pl) {
     pl->rows = 64;
     pl->CH = a->head_dim <= 128 ? 64 : 32;
     pl->TS = pl->rows / grp;
-    pl->smem = (size_t)(pl->rows + 2 * pl->CH) * (a->head_dim + 8) * 2 + (size_t)(groups + 1) * 4 + 128;
+    pl->smem = (size_t)(pl->rows + 2 * pl->CH) * (a->head_dim + 8) * 2 + ragged_table_bytes(groups);
   }
   pl->ctas = a->num_ctas;
   if (pl->ctas <= 0) {

@@ -56,13 +56,12 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
   uint16_t* sk = sq + C::kRows * LD;
   uint16_t* sv = sk + CH * LD;
   int32_t* table = reinterpret_cast<int32_t*>(sv + CH * LD);
-  int32_t* warp_tmp = table + p.G + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int gq = lane >> 2, tq = lane & 3;
 
   griddep_wait();
   griddep_launch();
-  ragged_table(p, table, warp_tmp);
+  ragged_table(p, table);
   ragged_rows_without_keys<D, QT>(p);
   const int W = table[p.G];
   const int ctas = W < (int)gridDim.x ? W : (int)gridDim.x;

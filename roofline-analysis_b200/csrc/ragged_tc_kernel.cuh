@@ -16,15 +16,15 @@
 // Warps 0-3 and 4-7: softmax and output of stream 0 and 1 (thread = row =
 // TMEM lane, so maximum, sum and rescaling need no other thread).  Warp 8:
 // one thread issues the MMAs of both streams in turn, which keeps one stream's
-// products beside the other's softmax.  Warp 10: TMA.  Warp 11: the last V
-// tile of a sequence, see below.  e4m3 caches: warps 12-15 convert each raw
+// products beside the other's softmax.  Warp 10: TMA (head_dim 128, 16 bits: K
+// only, and warp 9 V).  Warp 11: the last V tile of a sequence, see below.  e4m3 caches: warps 12-15 convert each raw
 // tile to fp16 (exact) into the swizzled layout the MMAs read; q and P are then
 // fp16 too.  The softmax warps get registers of the others (setmaxnreg).
 //
 // The maximum is lazy: it moves only when a score exceeds it by 2^8, so P <=
-// 256 and O is rescaled (a TMEM round trip) rarely.  So the weights are
-// computed with the old maximum at once, while the chunk's own maximum is
-// found beside them, and computed again in the rare case that it moves.
+// 256 and O is rescaled (a TMEM round trip) rarely: a chunk that leaves it, or
+// sets it first, goes from S to P in registers, any other takes the general
+// step.
 //
 // Keys past the end: their pages are not loaded, their scores are masked, and
 // warp 11 (e4m3: the conversion) zeroes their V rows, which may hold anything,
@@ -48,6 +48,10 @@ struct RaggedTc {
   static constexpr uint32_t kRaw = 128 * D;          // e4m3 tile [128 keys][D]
   static constexpr int kSlots = (kFp8 ? 98304 : 131072) / kTile;   // K and V alternate
   static constexpr int kRawSlots = kFp8 ? 32768 / kRaw : 0;
+  // K and V loads from a warp each: 866 -> 832 us for 16 requests of up to 1024 x
+  // 6500 tokens at head_dim 128; at head_dim 64, whose tiles are half as large, it
+  // cost 5 %.
+  static constexpr bool kTwoLoaders = D == 128 && !kFp8;
   static constexpr uint32_t kStage = 2048;           // output staging of a softmax warp
   static constexpr int kThreads = kFp8 ? 512 : 384;
   // Registers per thread, softmax and others: 256 x kRegSm + (kThreads - 256) x
@@ -62,8 +66,8 @@ struct RaggedTc {
   // full, empty, tail [slots]; raw full, empty; q, s, p, o full [2]; drain
   static constexpr int kBars = 3 * kSlots + 2 * kRawSlots + 9;
   static constexpr uint32_t kOffTmem = kOffBar + kBars * 8;
-  static constexpr uint32_t kOffTable = kOffTmem + 16;
-  static constexpr size_t smem(int groups) { return kOffTable + (size_t)(groups + 1 + 32) * 4 + 1024; }
+  static constexpr uint32_t kOffTable = kOffTmem + 16;   // (TMEM address, failure flag)
+  static constexpr size_t smem(int groups) { return kOffTable + ragged_table_bytes(groups) + 1024; }
 };
 
 // 32 lanes x 32 columns: register j of thread t is lane t (of the warp's
@@ -151,7 +155,9 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   int32_t* table = reinterpret_cast<int32_t*>(smem + C::kOffTable);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  volatile int* failed = reinterpret_cast<int*>(tmem_slot + 1);   // a wait ran out of time
   if (threadIdx.x == 0) {
+    *failed = 0;
     for (int i = 0; i < NS; ++i) {
       mbar_init(full + i, F8 ? 4 : 1);
       mbar_init(empty + i, 1);
@@ -183,7 +189,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   tc_fence_before();
   griddep_wait();                            // (everything above overlaps the kernel before)
   griddep_launch();
-  ragged_table(p, table, table + p.G + 1);   // ends with __syncthreads
+  ragged_table(p, table);                    // ends with __syncthreads
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   ragged_rows_without_keys<D, QT>(p);
@@ -198,7 +204,9 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     for (int i = 0; i < 64; ++i)   // the clock is read only after some polls
       if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, mla_wait(bar, parity, p.status, p.wait_ns));
+    const bool done = __all_sync(0xffffffffu, mla_wait(bar, parity, p.status, p.wait_ns));
+    if (!done) *failed = 1;
+    return done;
   };
   // One arrival per warp, behind what all its lanes did.
   auto arrive = [&](uint64_t* bar) {
@@ -498,7 +506,9 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       auto wait1 = [&](uint64_t* bar, uint32_t parity) -> bool {
         for (int i = 0; i < 64; ++i)
           if (mbar_try_wait(bar, parity)) return true;
-        return mla_wait(bar, parity, p.status, p.wait_ns);
+        const bool done = mla_wait(bar, parity, p.status, p.wait_ns);
+        if (!done) *failed = 1;
+        return done;
       };
       uint32_t ring = 0;                         // ring position of the piece's first K
       uint32_t np[2] = {0, 0}, nq[2] = {0, 0};
@@ -549,8 +559,11 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       wait1(drain, 0);
     }
     __syncwarp();
-  } else if (warp == 10) {
-    // ---------------- TMA producer ----------------
+  } else if (warp == 10 || (warp == 9 && C::kTwoLoaders)) {
+    // ---------------- TMA producer(s) ----------------
+    // Two of them both walk the whole ring.  Neither can be two phases of a
+    // slot's barrier ahead: the tile that it loaded last waited for one that is
+    // consumed after those.
     if (!p.no_loads) {
       constexpr int N = F8 ? NR : NS;
       constexpr int PB = F8 ? 1 : C::kBlk;       // boxes per granule
@@ -585,24 +598,22 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           }
           const int left = min(CH, w.len - c * CH);
           const uint32_t tx = (uint32_t)((left + granule - 1) / granule * granule) * kBox * PB;
-          const int next = page_of(c + 1);
+          const int next = page_of(c + 1), off = t % p.P;
           for (int u = 0; u < 2 * w.heads; ++u, ++n) {   // K of each head, V of each head
             const uint32_t slot = n % N;
             const bool is_v = u >= w.heads;
+            if (C::kTwoLoaders && is_v != (warp == 9)) continue;
             if (!wait(eb + slot, ((n / N) & 1u) ^ 1u)) { ok = false; break; }
             uint64_t* bar = !F8 && is_v && left < CH ? tail + slot : fb + slot;
             if (lane == 0) mbar_arrive_expect_tx(bar, tx);
             __syncwarp();
             if (load)
               tma_load_4d(smem + base + slot * bytes + (uint32_t)(blk * 16384 + gr * granule * (int)kBox),
-                          is_v ? &tmap_v : &tmap_k, bar, blk * 64, t % p.P, w.h + (is_v ? u - w.heads : u), page, policy);
+                          is_v ? &tmap_v : &tmap_k, bar, blk * 64, off, w.h + (is_v ? u - w.heads : u), page, policy);
           }
           page = next;
         }
       }
-      // Copies still in flight land before the block ends.
-      for (uint32_t i = n > (uint32_t)N ? n - N : 0; i < n; ++i)
-        if (!wait(fb + i % N, (i / N) & 1u)) break;
     }
   } else if (warp == 11) {
     // ---------------- last V tile of a sequence: zero the rows behind it ----------------
@@ -677,6 +688,12 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (*failed) {
+    // Every copy of a block that came through has been consumed; of one that
+    // gave up, those in flight land now.
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) {}
+  }
   if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

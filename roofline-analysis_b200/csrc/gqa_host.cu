@@ -290,14 +290,16 @@ static int launch_t(const GqaPlan& pl, const CUtensorMap& tk, const CUtensorMap&
 template <int D, int KIND, typename QT, bool VL = false>
 static int launch_mma(const GqaPlan& pl, const CUtensorMap& tk, const CUtensorMap& tv,
                       const GqaParams& p, cudaStream_t st, int flags) {
+  auto combine = gqa_combine_kernel<D, QT>;
+  auto run = [&](auto kernel) { return launch_k(kernel, combine, pl, tk, tv, p, st, flags); };
   if (pl.np == 2) {
     if constexpr (D >= 192) return B2D_ERR_UNSUPPORTED;
     else
-      return launch_k(gqa_mma_kernel<D, KIND, QT, 2, VL>, gqa_combine_kernel<D, QT>, pl, tk, tv,
-                      p, st, flags);
+      return p.out_f32 ? run(gqa_mma_kernel<D, KIND, QT, 2, VL, true>)
+                       : run(gqa_mma_kernel<D, KIND, QT, 2, VL>);
   }
-  return launch_k(gqa_mma_kernel<D, KIND, QT, 1, VL>, gqa_combine_kernel<D, QT>, pl, tk, tv, p,
-                  st, flags);
+  return p.out_f32 ? run(gqa_mma_kernel<D, KIND, QT, 1, VL, true>)
+                   : run(gqa_mma_kernel<D, KIND, QT, 1, VL>);
 }
 
 template <int D, int KIND, typename QT>

@@ -557,7 +557,7 @@ __global__ void __maxnreg__(B2D_GQA_MAXNREG)
 // output of a batch of U segments are loaded together, folded in with a
 // running maximum.  The partials of other CTAs are read past L1 (__ldcg),
 // after the acquire fence of the arrival counter.
-template <int D, typename QT>
+template <int D, typename QT, bool F32>
 __device__ __forceinline__ void warp_merge_heads(const GqaParams& p, int b, int hg, int HQC,
                                                  int qh_row0, int nh, int64_t seg0, int nseg) {
   constexpr float kLn2 = 0.69314718055994530942f;
@@ -609,7 +609,7 @@ __device__ __forceinline__ void warp_merge_heads(const GqaParams& p, int b, int 
       const int qh = hg * HQC + qh_row;
       const int64_t at = (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + hl * EPL;
       const float inv = 1.f / wsum;
-      if (p.out_f32 != nullptr) {
+      if constexpr (F32) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) p.out_f32[at + e] = acc[e] * inv;
       } else {
@@ -624,7 +624,7 @@ __device__ __forceinline__ void warp_merge_heads(const GqaParams& p, int b, int 
 
 // One warp writes out = 0, lse = -inf for query heads [qh_row0, qh_row0 + nh)
 // of a zero-length row (b, hg).
-template <int D, typename QT>
+template <int D, typename QT, bool F32>
 __device__ __forceinline__ void warp_zero_heads(const GqaParams& p, int b, int hg, int HQC,
                                                 int qh_row0, int nh) {
   constexpr int EPL = D / 32;
@@ -632,7 +632,7 @@ __device__ __forceinline__ void warp_zero_heads(const GqaParams& p, int b, int h
   for (int hw = 0; hw < nh; ++hw) {
     const int qh = hg * HQC + qh_row0 + hw;
     const int64_t at = (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + lane * EPL;
-    if (p.out_f32 != nullptr) {
+    if constexpr (F32) {
 #pragma unroll
       for (int e = 0; e < EPL; ++e) p.out_f32[at + e] = 0.f;
     } else {

@@ -134,7 +134,9 @@ __device__ __forceinline__ float q_at(const QT* qrow, bool valid, int dim) {
 // ldmatrix's 8 token rows are 16 bytes apart); V tiles arrive transposed
 // ([head][D][16 tokens], 32-byte rows, no swizzle) and feed the P.V product
 // through plain (non-transposing) ldmatrix.
-template <int D, int KIND, typename QT, int NP, bool VL = false>
+// F32: out goes to p.out_f32 (a kernel of its own: the choice at run time cost
+// the FP8 decode 0.8 %).
+template <int D, int KIND, typename QT, int NP, bool VL = false, bool F32 = false>
 __global__ void __launch_bounds__(32 * 9, 1)
     gqa_mma_kernel(const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v, const GqaParams p) {
@@ -188,8 +190,8 @@ __global__ void __launch_bounds__(32 * 9, 1)
     for (int r = cta; r < R; r += gridDim.x) {
       if (row_start[r + 1] != row_start[r]) continue;
       const int b = r / p.HG;
-      warp_zero_heads<D, QT>(p, b, r - b * p.HG, p.HK * p.group,
-                             hk_w * p.group + (warp - hk_w * p.WPH) * gw_w, gw_w);
+      warp_zero_heads<D, QT, F32>(p, b, r - b * p.HG, p.HK * p.group,
+                                  hk_w * p.group + (warp - hk_w * p.WPH) * gw_w, gw_w);
     }
   }
   if (W == 0 || cta >= G) return;
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
         const int qh_row = qh_row0 + hw;
         if (cf == cl) {
           const int64_t at = (int64_t)b * p.o_sb + (int64_t)(hg * HQC + qh_row) * p.o_sh;
-          if (p.out_f32 != nullptr) {
+          if constexpr (F32) {
             float* dst = p.out_f32 + at;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
       old = __shfl_sync(0xffffffffu, old, 0);
       if (old == cl - cf) {
         __syncwarp();   // lane 0's acquire, then the other lanes' loads
-        warp_merge_heads<D, QT>(p, b, hg, HQC, qh_row0, GW, (int64_t)row + cf, cl - cf + 1);
+        warp_merge_heads<D, QT, F32>(p, b, hg, HQC, qh_row0, GW, (int64_t)row + cf, cl - cf + 1);
         if (lane == 0) *cnt = 0;
       }
     }

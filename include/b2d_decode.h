@@ -257,8 +257,8 @@ int b2d_append_kv(const b2d_append_args* args, void* stream);
  *              max_pages_per_seq]
  *   lse        [num_tokens, num_q_heads] fp32 (may be NULL)
  * A request without states yields out = 0 and lse = -inf; tokens behind
- * query_starts[num_groups] are left as they were.  head_dim 64, 128, 192 and
- * 256, group (num_q_heads / num_kv_heads) <= 32.
+ * query_starts[num_groups] are left as they were.  out overlaps no input.
+ * head_dim 64, 128, 192 and 256, group (num_q_heads / num_kv_heads) <= 32.
  */
 typedef struct b2d_cross_args {
   const void* q;
@@ -308,7 +308,8 @@ int b2d_cross_attention(const b2d_cross_args* args, void* stream);
  *   group_starts int32 [num_groups + 1]: group g holds sequences
  *              [group_starts[g], group_starts[g + 1]); sequences outside
  *              every group have no prefix.  NULL: one group with all.
- * Either part may be empty; both: out = 0, lse = -inf.  num_groups <= 4096.
+ * Either part may be empty; both: out = 0, lse = -inf.  out overlaps no input.
+ * num_groups <= 4096.
  */
 typedef struct b2d_shared_prefix_args {
   b2d_gqa_args own;
@@ -369,7 +370,8 @@ int b2d_merge_states(const b2d_merge_args* args, void* stream);
  * max_tokens are too few, block_table stays, seqlens_out = cache_seqlens,
  * free_count_out = *free_count, all slots are -1, query_starts are 0, and the
  * status word reports B2D_ERR_DEVICE_CAPACITY.  Negative lengths and counts
- * count as 0.  num_requests <= 16384.  No counterpart in the reference.
+ * count as 0.  num_requests <= 16384, max_tokens <= 2^30, max_pages_per_seq *
+ * page_size < 2^31.  No counterpart in the reference.
  */
 typedef struct b2d_plan_append_args {
   const int32_t* cache_seqlens;

@@ -91,6 +91,8 @@ def plan_append(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pag
             max_tokens = bsz
         else:
             raise ValueError(f"{where}: new_tokens needs max_tokens or slot_mapping")
+    if max_tokens < 0:
+        raise ValueError(f"{where}: max_tokens must not be negative")
     if slot_mapping is None:
         slot_mapping = cache_seqlens.new_empty((max_tokens,), dtype=torch.int64)
     else:

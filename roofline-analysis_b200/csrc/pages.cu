@@ -239,6 +239,16 @@ static int check_header(const void* ws, size_t bytes) {
   return ((uintptr_t)ws & 255) ? B2D_ERR_ALIGNMENT : B2D_OK;
 }
 
+// Whether lens_out or count_out overlaps an array that the blocks read.
+static bool updates_inputs(const PagesParams& p) {
+  auto overlap = [](const void* out, const void* in, size_t n) {
+    return in && (uintptr_t)out + n > (uintptr_t)in && (uintptr_t)in + n > (uintptr_t)out;
+  };
+  const size_t rows = (size_t)p.B * 4;
+  return overlap(p.lens_out, p.lens, rows) || overlap(p.lens_out, p.new_tokens, rows) ||
+         overlap(p.count_out, p.free_count, 4);
+}
+
 }  // namespace b2d
 
 using namespace b2d;
@@ -273,13 +283,7 @@ extern "C" int b2d_plan_append(const b2d_plan_append_args* a, void* stream) {
   p.P = a->page_size;
   p.max_tokens = a->max_tokens;
   p.capacity = a->free_capacity;
-  // Any output array that starts inside an input one counts as that one.
-  auto inside = [](const void* out, const void* in, size_t n) {
-    return (uintptr_t)out + n > (uintptr_t)in && (uintptr_t)in + n > (uintptr_t)out;
-  };
-  const size_t rows = (size_t)p.B * 4;
-  p.in_place = inside(p.lens_out, p.lens, rows) || inside(p.count_out, p.free_count, 4) ||
-               (p.new_tokens && inside(p.lens_out, p.new_tokens, rows));
+  p.in_place = updates_inputs(p);
   int sms = 0;
   if (device_sm_count(&sms)) return B2D_ERR_CUDA;
   const size_t smem = (size_t)p.B * 12;
@@ -316,13 +320,7 @@ extern "C" int b2d_release_pages(const b2d_release_args* a, void* stream) {
   p.max_pages = a->max_pages_per_seq;
   p.P = a->page_size;
   p.capacity = a->free_capacity;
-  // Any output array that starts inside an input one counts as that one.
-  auto inside = [](const void* out, const void* in, size_t n) {
-    return (uintptr_t)out + n > (uintptr_t)in && (uintptr_t)in + n > (uintptr_t)out;
-  };
-  const size_t rows = (size_t)p.B * 4;
-  p.in_place = inside(p.lens_out, p.lens, rows) || inside(p.count_out, p.free_count, 4) ||
-               (p.new_tokens && inside(p.lens_out, p.new_tokens, rows));
+  p.in_place = updates_inputs(p);
   int sms = 0;
   if (device_sm_count(&sms)) return B2D_ERR_CUDA;
   const size_t smem = (size_t)p.B * 4;

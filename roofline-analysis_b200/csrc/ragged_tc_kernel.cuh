@@ -17,9 +17,10 @@
 // TMEM lane, so maximum, sum and rescaling need no other thread).  Warp 8:
 // one thread issues the MMAs of both streams in turn, which keeps one stream's
 // products beside the other's softmax.  Warp 10: TMA (head_dim 128, 16 bits: K
-// only, and warp 9 V).  Warp 11: the last V tile of a sequence, see below.  e4m3 caches: warps 12-15 convert each raw
-// tile to fp16 (exact) into the swizzled layout the MMAs read; q and P are then
-// fp16 too.  The softmax warps get registers of the others (setmaxnreg).
+// only, and warp 9 V).  Warp 11: the last V tile of a sequence, see below.
+// e4m3 caches: warps 12-15 convert each raw tile to fp16 (exact) into the
+// swizzled layout the MMAs read; q and P are then fp16 too.  The softmax warps
+// get registers of the others (setmaxnreg).
 //
 // The maximum is lazy: it moves only when a score exceeds it by 2^8, so P <=
 // 256 and O is rescaled (a TMEM round trip) rarely: a chunk that leaves it, or
@@ -310,11 +311,13 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
                                    : (int64_t)d.segment(blockIdx.x) * p.rows + st * p.TS * p.grp + r;
           const int64_t my_row = (int64_t)tok * p.Hq + head;
           const int piece = lane & 3, row4 = lane >> 2;
-          auto piece_at = [&](int row, int q) { return stage + (uint32_t)(row * 64 + ((q ^ ((row >> 1) & 3)) << 4)); };
+          auto piece_at = [&](int row, int q) {
+            return stage + (uint32_t)(row * 64 + ((q ^ ((row >> 1) & 3)) << 4));
+          };
           uint32_t v[16];
           float4 z[4];                             // own parts of the next columns
           auto load_own = [&](int c) {
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float ow = __shfl_sync(0xffffffffu, own, 8 * i + row4);
               const int64_t orow = __shfl_sync(0xffffffffu, my_row, 8 * i + row4);
@@ -330,20 +333,20 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           };
           tmem_ld16(t_o, v);
           if (join) load_own(0);
-  #pragma unroll 1
+#pragma unroll 1
           for (int c = 0; c < D; c += 16) {
             tmem_wait_ld();
-  #pragma unroll
+#pragma unroll
             for (int q = 0; q < 4; ++q) {
               float f[4];
-  #pragma unroll
+#pragma unroll
               for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[4 * q + e]) * inv;
               sts128(piece_at(lane, q), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]),
                                                    __float_as_uint(f[2]), __float_as_uint(f[3])));
             }
             if (c + 16 < D) tmem_ld16(t_o + (uint32_t)(c + 16), v);
             __syncwarp();
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int rl = 8 * i + row4, cc = c + 4 * piece;
               uint4 y = lds128(piece_at(rl, piece));

@@ -151,6 +151,7 @@ static RaggedParams params_of(const b2d_cross_args* a, const RaggedPlan& pl, uin
   p.CH = pl.CH;
   p.rows = pl.rows;
   p.pairs = pl.tc ? 1 : 0;
+  p.spread = (int64_t)a->num_tokens / pl.TS * a->num_kv_heads >> p.pairs >= 2 * (int64_t)pl.ctas;
   p.scale = a->softmax_scale * 1.4426950408889634f;
   return p;
 }

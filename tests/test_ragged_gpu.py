@@ -190,6 +190,25 @@ def test_cross_nan_and_infinity_in_keys(cuda, kv, num_ctas):
         assert torch.equal(out[:40, :2], clean[:40, :2]) and torch.equal(out[40:], clean[40:]), pos
 
 
+@pytest.mark.parametrize("num_ctas", [1, 2, 3, 5, 11])
+@pytest.mark.parametrize("d,P", [(64, 16), (128, 5)])
+def test_cross_several_items_per_block(cuda, d, P, num_ctas):
+    """Many tiles of long sequences to a block (the order of items on the work
+    line changes with their number per block), odd tile counts, a cut or none."""
+    lens, tq = [2100, 2048, 10, 4000], [700, 130, 3, 260]
+    gen, k, v, _, _, bt = make(cuda, 80, lens, P, 3, d, BF, "NHD")
+    starts = [0]
+    for n in tq:
+        starts.append(starts[-1] + n)
+    q = torch.randn(starts[-1], 6, d, generator=gen, device=cuda).to(BF)
+    st = torch.tensor(starts, dtype=torch.int32, device=cuda)
+    kl = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    out, lse = b200decode.cross_attention(q, k, v, kl, bt, query_starts=st, num_ctas=num_ctas)
+    ref = cross_reference(q, k, v, None, None, bt, starts, lens, d ** -0.5, "NHD")
+    check(out, ref[0], ref[2], u_of(BF), "out")
+    check_lse(lse, ref[1], ref[3])
+
+
 def test_cross_fuzz(cuda):
     """Random shapes of every kind against the reference."""
     import random

@@ -366,7 +366,7 @@ def merge_states(outs: torch.Tensor, lses: torch.Tensor, *, out: Optional[torch.
     index = outs.get_device()
     _one_device(where, index, lses, out, lse)
     n, t, h, d = shape
-    given = out is not None or lse is not None
+    given = [x for x in (out, lse) if x is not None]
     if out is None:
         out = outs.new_empty((t, h, d))
     else:
@@ -379,7 +379,7 @@ def merge_states(outs: torch.Tensor, lses: torch.Tensor, *, out: Optional[torch.
         raise ValueError(f"{where}: lse must be fp32 [{t}, {h}]")
     if given and out.numel():
         (o0, o1), (l0, l1) = _span(outs), _span(lses)
-        for x in (out, lse):
+        for x in given:
             first, end = _span(x)
             if (first < o1 and o0 < end) or (first < l1 and l0 < end):
                 raise ValueError(f"{where}: out or lse overlaps an input")

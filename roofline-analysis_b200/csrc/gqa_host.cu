@@ -241,13 +241,16 @@ static int launch_k(Kern kern, void (*combine)(const GqaParams, int, int), const
   // rows (small batches, rows over ~100 CTAs) the multi-warp combine kernel
   // spreads the merges instead.  B2D_GQA_FUSED_MERGE=0/1 forces either.
   static const int fused_env = env_int("B2D_GQA_FUSED_MERGE", -1);
-  // The fp32 output of a shared-prefix call is merged in the kernel only where no
-  // row has more than one chunk (nothing to merge) or rows outnumber CTAs: its
-  // rows are short, so that merging is much of the kernel.  Whole call, 1024 shared keys, 32
-  // on 8 heads, combine / in the kernel: 8 sequences with 16 own keys 27.5 / 25.1
-  // us, 512 32.1 / 36.6; 67 with 600 57.0 / 60.2; 256 with 600 136.7 / 135.8.
-  const int64_t row_keys = (int64_t)p.max_pages * p.P;
-  const bool in_kernel = p.out_f32 != nullptr ? R >= ctas || row_keys <= p.T : (int64_t)R * 7 >= ctas;
+  // The fp32 output of a shared-prefix call is merged in the kernel whenever no
+  // row has more than kMaxPieces pieces, because the prefix kernel, which starts
+  // while this one runs, hides the merge but waits for a combine launch.  Whole
+  // call, 1024 shared keys, 32 on 8 heads, combine / in the kernel: 4 sequences
+  // with 256 own keys 31.4 / 26.1 us, 2048 (37 pieces) 32.8 / 37.2; 32 with 600
+  // 44.4 / 37.8; 256 with 600 135.6 / 132.0.
+  constexpr int kMaxPieces = 24;
+  const int64_t row_chunks = ((int64_t)p.max_pages * p.P + p.T - 1) / p.T;
+  const bool in_kernel = (int64_t)R * 7 >= ctas ||
+                         (p.out_f32 != nullptr && (row_chunks <= kMaxPieces || (int64_t)R * kMaxPieces >= ctas));
   const bool fused = pl.mma && (fused_env >= 0 ? fused_env != 0 : in_kernel) &&
                      (int64_t)R * p.NW <= kMergeCounters;
   if (pl.launch_count != nullptr) {

@@ -303,6 +303,7 @@ __device__ __forceinline__ void ragged_row_without_keys(const RaggedParams& p, i
   const int lane = threadIdx.x & 31;
   StateMerge<EPL> m;
   if (p.own_o != nullptr) {
+    griddep_wait();
     const int64_t row = (int64_t)t * p.Hq + h;
     float o[EPL];
     load_lane<EPL>(p.own_o + row * D + lane * EPL, o);

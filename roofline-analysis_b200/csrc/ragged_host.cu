@@ -156,8 +156,8 @@ static RaggedParams params_of(const b2d_cross_args* a, const RaggedPlan& pl, uin
   return p;
 }
 
-// Launch whose prologue may overlap the kernel before it on the stream (the
-// kernel itself waits for that one's end before it touches global memory).
+// Launch whose start may overlap the kernel before it on the stream (the kernel
+// itself waits for that one's end before it reads what it wrote).
 template <typename... P, typename... A>
 static int launch_overlapped(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
                              A... args) {

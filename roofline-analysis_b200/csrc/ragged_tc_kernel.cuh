@@ -188,7 +188,11 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
     prefetch_tmap(&tmap_v);
   }
   tc_fence_before();
-  griddep_wait();                            // (everything above overlaps the kernel before)
+  // Everything above overlaps the kernel before.  Shared prefix: that one is the
+  // own-token decode, all of whose blocks have seen its inputs complete before
+  // they let this kernel start, so only its outputs are waited for, where they
+  // are read (and before the block ends, for the merge).
+  if (p.own_o == nullptr) griddep_wait();
   griddep_launch();
   ragged_table(p, table);                    // ends with __syncthreads
   tc_fence_after();
@@ -298,6 +302,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           const int tok = d.t0 + d.first(st, p.TS) + tq, head = d.head(st) * p.grp + hq;
           const bool join = whole && p.own_o != nullptr;
           float own = 0.f;                         // weight of the sequence's own part
+          if (join) griddep_wait();
           if (join && r < nrows) {
             const float2 jw = join_weights(lse2, p.own_lse[(int64_t)tok * p.Hq + head], lse2);
             inv *= jw.x;
@@ -689,6 +694,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
       }
     }
   }
+  if (p.own_o != nullptr) griddep_wait();
   tc_fence_before();
   __syncthreads();
   if (*failed) {

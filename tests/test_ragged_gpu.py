@@ -282,6 +282,35 @@ def test_decode_shared_prefix(cuda, case, num_ctas):
     check_lse(lse, ref[1], ref[3])
 
 
+@pytest.mark.parametrize("plens,starts", [([100], [0, 6]), ([100, 0], [1, 4, 6])])
+def test_shared_prefix_shorter_than_own_tokens(cuda, plens, starts):
+    """The prefix part is done long before the own tokens are: calls one after
+    another in one workspace, eager and captured, equal calls on their own."""
+    lens, d, P = [30000, 9000, 0, 12000, 17, 5000], 128, 16
+    gen, k, v, _, _, both = make(cuda, 140, plens + lens, P, 2, d, BF, "NHD")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    pl, st, ol, pbt, bt = i32(plens), i32(starts), i32(lens), both[:len(plens)], both[len(plens):]
+    qs = [torch.randn(6, 8, d, generator=gen, device=cuda).to(BF) for _ in range(4)]
+    call = lambda q: b200decode.decode_shared_prefix(q, k, v, pl, pbt, ol, bt, group_starts=st)  # noqa: E731
+    alone = []
+    for q in qs:
+        alone.append(call(q))
+        torch.cuda.synchronize()
+    ref = shared_reference(qs[0], k, v, None, None, pbt, plens, bt, lens, starts, d ** -0.5, "NHD")
+    check(alone[0][0], ref[0], ref[2], u_of(BF), "out")
+    check_lse(alone[0][1], ref[1], ref[3])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = [call(q) for q in qs]
+    for _ in range(5):
+        eager = [call(q) for q in qs]
+        graph.replay()
+        torch.cuda.synchronize()
+        for (o, l), (eo, el), (ho, hl) in zip(alone, eager, held):
+            # (which warp merges a cut row's pieces does not change their order)
+            assert torch.equal(o, eo) and torch.equal(l, el) and torch.equal(o, ho) and torch.equal(l, hl)
+
+
 def test_shared_prefix_of_one_table(cuda):
     """One table whose rows begin with the same pages, cut by columns into the
     two tables; q [B, 1, Hq, D]; the result is decode()'s over whole rows."""

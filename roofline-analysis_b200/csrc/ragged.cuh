@@ -65,6 +65,7 @@ struct RaggedParams {
   int64_t lse_st;
   const float* own_o;           // shared prefix: the part over each sequence's own tokens, [T, Hq, D]
   const float* own_lse;         // fp32 and [T, Hq] natural log, to be joined with; else null
+  int beside;                   // 1: start while the kernel that writes the own parts still runs
   float* seg_o;                 // [2 * CTAs][tile rows][D] fp32, normalised
   float* seg_lse;               // [2 * CTAs][tile rows], log2 units
   int32_t* cuts;                // [CTAs][8]: the item that each CTA begins and does not finish

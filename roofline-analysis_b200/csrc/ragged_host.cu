@@ -418,5 +418,7 @@ extern "C" int b2d_decode_shared_prefix(const b2d_shared_prefix_args* a, void* s
   RaggedParams p = params_of(&c, pl, ws + lay.off_part);
   p.own_o = own_o;
   p.own_lse = own_lse;
+  // (a wait with a short limit must not run while the own-token decode does)
+  p.beside = p.wait_ns >= kWaitLimitNs;
   return launch_both(&c, pl, p, st);
 }

@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   // own-token decode, all of whose blocks have seen its inputs complete before
   // they let this kernel start, so only its outputs are waited for, where they
   // are read (and before the block ends, for the merge).
-  if (p.own_o == nullptr) griddep_wait();
+  if (!p.beside) griddep_wait();
   griddep_launch();
   ragged_table(p, table);                    // ends with __syncthreads
   tc_fence_after();

@@ -299,6 +299,9 @@ def test_shared_prefix_shorter_than_own_tokens(cuda, plens, starts):
     ref = shared_reference(qs[0], k, v, None, None, pbt, plens, bt, lens, starts, d ** -0.5, "NHD")
     check(alone[0][0], ref[0], ref[2], u_of(BF), "out")
     check_lse(alone[0][1], ref[1], ref[3])
+    # A wait limit below the default: one part after the other.
+    limited = b200decode.decode_shared_prefix(qs[1], k, v, pl, pbt, ol, bt, group_starts=st, wait_limit_us=500000)
+    assert all(torch.equal(x, y) for x, y in zip(limited, alone[1]))
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         held = [call(q) for q in qs]

@@ -186,7 +186,9 @@ static int make_plan(const b2d_gqa_args* a, GqaPlan* pl) {
     if (tmax > 256) tmax = 256;
     pl->T = largest_divisor_leq(a->page_size, tmax);
   }
-  pl->stage_bytes = (uint32_t)(pl->T * row_bytes);
+  // (an e4m3 tile of one head of 64 and an odd number of tokens ends between
+  // two addresses that a TMA copy may start at)
+  pl->stage_bytes = (uint32_t)align_up((size_t)pl->T * row_bytes, 128);
   static const size_t ring = (size_t)env_int("B2D_GQA_RING_KB", (int)(kStageRingBytes / 1024)) * 1024;
   int stages = (int)(ring / (2 * (size_t)pl->stage_bytes));
   pl->stages = stages < 2 ? 2 : (stages > 8 ? 8 : stages);

@@ -70,7 +70,7 @@ struct GqaParams {
   int B, Hq, Hkv, group, HK, HG, P, T, stages, NW, WPH;
   int num_pages, max_pages;
   float scale_log2;        // softmax_scale * log2(e)
-  uint32_t stage_bytes;    // bytes of one K (or V) tile
+  uint32_t stage_bytes;    // from one K (or V) tile to the next: a multiple of 128, as TMA needs
 };
 
 // Exclusive block-wide scan of n_r = ceil(min(L_b, cap) / T) over R rows
@@ -289,7 +289,7 @@ __global__ void __maxnreg__(B2D_GQA_MAXNREG)
             ok = false;
           } else {
             uint8_t* kdst = tiles + (size_t)s * 2 * p.stage_bytes;
-            mbar_arrive_expect_tx(full + s, 2u * p.stage_bytes);
+            mbar_arrive_expect_tx(full + s, 2u * (uint32_t)(p.T * p.HK * D * ES));
             tma_load_4d(kdst, &tmap_k, full + s, 0, h0, off, page, policy);
             tma_load_4d(kdst + p.stage_bytes, &tmap_v, full + s, 0, h0, off, page, policy);
           }

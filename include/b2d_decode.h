@@ -370,7 +370,8 @@ int b2d_merge_states(const b2d_merge_args* args, void* stream);
  * max_tokens are too few, block_table stays, seqlens_out = cache_seqlens,
  * free_count_out = *free_count, all slots are -1, query_starts are 0, and the
  * status word reports B2D_ERR_DEVICE_CAPACITY.  Negative lengths and counts
- * count as 0.  num_requests <= 16384, max_tokens <= 2^30, max_pages_per_seq *
+ * count as 0.  A negative page taken from free_pages is written into the table,
+ * gives slots of -1 and is reported as B2D_ERR_DEVICE_BOUNDS.  num_requests <= 16384, max_tokens <= 2^30, max_pages_per_seq *
  * page_size < 2^31.  No counterpart in the reference.
  */
 typedef struct b2d_plan_append_args {
@@ -397,8 +398,11 @@ int b2d_plan_append(const b2d_plan_append_args* args, void* stream);
  * The reverse: requests with finished[b] != 0 give all their pages back.  In
  * request order, then page order, they are pushed onto free_pages behind
  * *free_count; seqlens_out of such a request is 0.  block_table is only
- * read.  When free_pages (free_capacity entries) has no room for all, nothing
- * changes and the status word reports B2D_ERR_DEVICE_CAPACITY.
+ * read.  When free_pages (free_capacity entries) has no room for all, or a
+ * finished request is longer than its row, nothing changes and the status word
+ * reports B2D_ERR_DEVICE_CAPACITY; when one of the pages is negative,
+ * B2D_ERR_DEVICE_BOUNDS (free_pages behind *free_count may then be
+ * overwritten, the lengths and the count are as before).
  */
 typedef struct b2d_release_args {
   const int32_t* cache_seqlens;

@@ -74,8 +74,9 @@ def plan_append(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pag
     themselves, so that a captured step continues the last one.  A step that
     does not fit (free pages, table columns or max_tokens) changes nothing:
     slots are -1, query_starts 0, lengths and free_count as before, and
-    check_device_status() raises B2D_ERR_DEVICE_CAPACITY.  Up to 16384
-    requests.  In a CUDA graph, pass `workspace` to read that status.
+    check_device_status() raises B2D_ERR_DEVICE_CAPACITY.  A negative page taken
+    from the pool gives slots of -1 and is reported (B2D_ERR_DEVICE_BOUNDS).  Up
+    to 16384 requests.  In a CUDA graph, pass `workspace` to read that status.
     """
     where = "plan_append"
     bsz = _pool(where, cache_seqlens, block_table, free_pages, free_count, page_size)
@@ -133,8 +134,10 @@ def release_pages(cache_seqlens: torch.Tensor, block_table: torch.Tensor, finish
     seqlens_out and free_count_out.  Keep the pages of a shared prefix out of
     the rows (as decode_shared_prefix() has them): a row's pages are given back
     once for each request that holds them.  When free_pages has no room for
-    all, nothing changes and check_device_status() raises
-    B2D_ERR_DEVICE_CAPACITY."""
+    all, or a finished request is longer than its row, nothing changes and
+    check_device_status() raises B2D_ERR_DEVICE_CAPACITY; when one of the pages
+    is negative, B2D_ERR_DEVICE_BOUNDS (free_pages behind free_count may then
+    be overwritten)."""
     where = "release_pages"
     bsz = _pool(where, cache_seqlens, block_table, free_pages, free_count, page_size)
     if finished.dtype is not torch.bool or finished.shape != (bsz,) or not finished.is_contiguous():

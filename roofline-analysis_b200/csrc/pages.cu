@@ -40,7 +40,7 @@ struct PagesParams {
   int* status;
   int* arrivals;
   int B, max_pages, P, max_tokens, capacity;
-  int in_place;                 // an output is an input: written by the last block
+  int in_place;                 // append: an output is an input, written by the last block
 };
 
 __device__ __forceinline__ int64_t pages_of(int64_t tokens, int P) { return (tokens + P - 1) / P; }
@@ -105,16 +105,19 @@ __device__ __forceinline__ int request_of(const int32_t* start, int B, int i) {
 }
 
 // True in the block that arrives last: every other block has read its inputs.
-__device__ __forceinline__ bool last_block(int* arrivals) {
-  __shared__ int last;
-  __syncthreads();
+// `bad`: whether a thread of this block, on return of any block, has set it (the
+// blocks that have are counted above the arrivals; there are at most 65535).
+__device__ __forceinline__ bool last_block(int* arrivals, bool& bad) {
+  __shared__ int seen;
+  bad = __syncthreads_or(bad);
   if (gridDim.x == 1) return true;
   if (threadIdx.x == 0) {
-    last = atomic_add_acq_rel_gpu(arrivals, 1) == (int)gridDim.x - 1;
-    if (last) *arrivals = 0;
+    seen = atomic_add_acq_rel_gpu(arrivals, bad ? 0x10001 : 1);
+    if ((seen & 0xffff) == (int)gridDim.x - 1) *arrivals = 0;
   }
   __syncthreads();
-  return last != 0;
+  bad = bad || (seen >> 16) != 0;
+  return (seen & 0xffff) == (int)gridDim.x - 1;
 }
 
 __global__ void __launch_bounds__(kPageThreads) plan_append_kernel(const PagesParams p) {
@@ -179,10 +182,12 @@ __global__ void __launch_bounds__(kPageThreads) plan_append_kernel(const PagesPa
   }
   for (int k = first; k < np; k += step) {
     const int b = request_of(page_start, p.B, k);
-    const int have = (int)pages_of(lens[b], p.P);
-    p.table[b * p.table_stride + have + (k - page_start[b])] = p.free_pages[count - 1 - k];
+    const int have = (int)pages_of(lens[b], p.P), page = p.free_pages[count - 1 - k];
+    if (page < 0) record_status(p.status, kStatusBounds);
+    p.table[b * p.table_stride + have + (k - page_start[b])] = page;
   }
-  if (p.in_place ? !last_block(p.arrivals) : blockIdx.x != 0) return;
+  bool unused = false;
+  if (p.in_place ? !last_block(p.arrivals, unused) : blockIdx.x != 0) return;
   for (int b = tid; b < p.B; b += kPageThreads) p.lens_out[b] = fits ? lens[b] + new_of(p, b) : p.lens[b];
   if (tid == 0) {
     *p.count_out = fits ? count - np : count_in;
@@ -197,35 +202,39 @@ __global__ void __launch_bounds__(kPageThreads) release_pages_kernel(const Pages
   const int count_in = *p.free_count;
   const int per = (p.B + kPageThreads - 1) / kPageThreads;
   const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  bool in_table = true;   // no finished request is longer than its row
   auto given = [&](int b) -> int64_t {
     if (p.finished[b] == 0) return 0;
     const int64_t n = pages_of(length_of(p, b), p.P);
-    return n < p.max_pages ? n : p.max_pages;
+    in_table = in_table && n <= p.max_pages;
+    return n;
   };
   int64_t pages = 0, unused = 0, total, unused_total;
   for (int b = b0; b < b1; ++b) pages += given(b);
   block_scan2(pages, unused, total, unused_total);
   const int count = max(0, min(count_in, p.capacity));
-  const bool fits = total <= p.capacity - count;
+  bool fits = __syncthreads_and(in_table && total <= p.capacity - count);
   for (int b = b0; b < b1; ++b) {   // used only when the total fits 32 bits
     page_start[b] = (int)pages;
     pages += given(b);
   }
   __syncthreads();
   const int np = fits ? (int)total : 0;
+  bool negative = false;
   for (int k = blockIdx.x * kPageThreads + tid; k < np; k += gridDim.x * kPageThreads) {
     const int b = request_of(page_start, p.B, k);
-    p.free_pages[count + k] = p.table[b * p.table_stride + (k - page_start[b])];
+    const int page = p.table[b * p.table_stride + (k - page_start[b])];
+    negative = negative || page < 0;
+    p.free_pages[count + k] = page;
   }
-  if (p.in_place ? !last_block(p.arrivals) : blockIdx.x != 0) return;
+  if (!last_block(p.arrivals, negative)) return;
+  if (tid == 0 && !(fits && !negative)) record_status(p.status, fits ? kStatusBounds : kStatusCapacity);
+  fits = fits && !negative;
   for (int b = tid; b < p.B; b += kPageThreads) {
     const int L = p.lens[b];
     p.lens_out[b] = fits && p.finished[b] ? 0 : L;
   }
-  if (tid == 0) {
-    *p.count_out = fits ? count + np : count_in;
-    if (!fits) record_status(p.status, kStatusCapacity);
-  }
+  if (tid == 0) *p.count_out = fits ? count + np : count_in;
 }
 
 // Blocks for `work` entries: one per 2048, at most one per SM.
@@ -320,7 +329,6 @@ extern "C" int b2d_release_pages(const b2d_release_args* a, void* stream) {
   p.max_pages = a->max_pages_per_seq;
   p.P = a->page_size;
   p.capacity = a->free_capacity;
-  p.in_place = updates_inputs(p);
   int sms = 0;
   if (device_sm_count(&sms)) return B2D_ERR_CUDA;
   const size_t smem = (size_t)p.B * 4;

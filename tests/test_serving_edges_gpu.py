@@ -56,3 +56,68 @@ def test_e4m3_tiles_of_any_number_of_bytes(cuda, hkv, grp, P, num_ctas):
         for (out, lse), ref in zip(got, (part[0], merge2(*part))):
             check(out[b:b + 1], ref[0], ref[2], u_of(BF), "out")
             check_lse(lse[b:b + 1], ref[1], ref[3])
+
+
+# ---------------------------------------------------------------- pages
+
+@pytest.mark.parametrize("B", [3, 900])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_release_of_a_negative_page_changes_nothing(cuda, B, in_place):
+    """A negative entry among the pages of a finished request never enters the
+    pool: the step is reported and changes no length, count or free page."""
+    P, width = 16, 7
+    bt = torch.arange(B * width, dtype=torch.int32, device=cuda).reshape(B, width)
+    lens = torch.full((B,), 100, dtype=torch.int32, device=cuda)      # all 7 pages
+    lens[1] = 33                                                      # 3 pages
+    bt[1, 3] = -8                                                     # (not one of them)
+    fin = torch.ones(B, dtype=torch.bool, device=cuda)
+    fin[0] = False
+    bt[0, 2] = -1                                                     # (not finished)
+    free = torch.full((B * width + 5,), -5, dtype=torch.int32, device=cuda)
+    free[:5] = i32([B * width + x for x in range(5)])
+    ws = b200decode.DecodeWorkspace(cuda)
+    for bad in (True, False):
+        table, sl, fr, cnt = bt.clone(), lens.clone(), free.clone(), i32([5])
+        if bad:
+            table[B - 1, 4] = -3
+        kw = dict(seqlens_out=sl, free_count_out=cnt) if in_place else {}
+        after, count = b200decode.release_pages(sl, table, fin, fr, cnt, P, workspace=ws, **kw)
+        torch.cuda.synchronize()
+        if bad:
+            with pytest.raises(b200decode.B2DError) as e:
+                b200decode.check_device_status(ws)
+            assert e.value.code == -7
+            assert torch.equal(after, lens) and int(count) == 5
+            assert torch.equal(fr[:5], free[:5])
+        else:
+            b200decode.check_device_status(ws)
+            given = [int(x) for b in range(1, B) for x in table[b, :3 if b == 1 else 7].tolist()]
+            assert int(count) == 5 + len(given) and fr[:int(count)].tolist() == free[:5].tolist() + given
+            assert after.tolist() == [100] + [0] * (B - 1)
+
+
+def test_release_of_a_length_beyond_the_table_changes_nothing(cuda):
+    bt = torch.arange(8, dtype=torch.int32, device=cuda).reshape(2, 4)
+    sl, free, cnt = i32([64, 65]), torch.zeros(8, dtype=torch.int32, device=cuda), i32([0])
+    ws = b200decode.DecodeWorkspace(cuda)
+    after, count = b200decode.release_pages(sl, bt, torch.tensor([True, True], device=cuda), free, cnt, 16, workspace=ws)
+    with pytest.raises(b200decode.B2DError) as e:
+        b200decode.check_device_status(ws)
+    assert e.value.code == -9
+    assert after.tolist() == [64, 65] and int(count) == 0 and (free == 0).all()
+    after, count = b200decode.release_pages(sl, bt, torch.tensor([True, False], device=cuda), free, cnt, 16, workspace=ws)
+    b200decode.check_device_status(ws)
+    assert after.tolist() == [0, 65] and free[:4].tolist() == [0, 1, 2, 3] and int(count) == 4
+
+
+def test_plan_append_reports_a_negative_page_of_the_pool(cuda):
+    free = i32([4, -6, 5])
+    ws = b200decode.DecodeWorkspace(cuda)
+    bt = torch.zeros(2, 2, dtype=torch.int32, device=cuda)
+    plan = b200decode.plan_append(i32([0, 0]), bt, free, i32([3]), 16, workspace=ws)
+    assert plan.slot_mapping.tolist() == [80, -1]
+    with pytest.raises(b200decode.B2DError) as e:
+        b200decode.check_device_status(ws)
+    assert e.value.code == -7
+    b200decode.plan_append(i32([0]), bt[:1], free, i32([3]), 16, workspace=ws)
+    b200decode.check_device_status(ws)

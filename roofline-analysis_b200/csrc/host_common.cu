@@ -86,12 +86,21 @@ int encode_tiled_map(CUtensorMap* map, CUtensorMapDataType dtype, int rank, cons
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return -1;
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  CUresult r = fn(map, dtype, (cuuint32_t)rank, const_cast<void*>(base),
-                  reinterpret_cast<const cuuint64_t*>(dims),
-                  reinterpret_cast<const cuuint64_t*>(strides_bytes),
-                  reinterpret_cast<const cuuint32_t*>(box), estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(map, dtype, (cuuint32_t)rank, const_cast<void*>(base),
+              reinterpret_cast<const cuuint64_t*>(dims),
+              reinterpret_cast<const cuuint64_t*>(strides_bytes),
+              reinterpret_cast<const cuuint32_t*>(box), estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r != CUDA_SUCCESS) {
+    // A host thread without a runtime call so far has no current context, which
+    // this driver call needs: selecting the device that it is on makes one current.
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   return r == CUDA_SUCCESS ? 0 : -1;
 }
 

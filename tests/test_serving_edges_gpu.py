@@ -121,3 +121,35 @@ def test_plan_append_reports_a_negative_page_of_the_pool(cuda):
     assert e.value.code == -7
     b200decode.plan_append(i32([0]), bt[:1], free, i32([3]), 16, workspace=ws)
     b200decode.check_device_status(ws)
+
+
+# ---------------------------------------------------------------- two calls at once
+
+def test_first_call_of_a_host_thread(cuda):
+    """A thread whose first CUDA call is one of these, on tensors that another
+    thread made."""
+    lens = [40, 300]
+    gen, k, v, _, _, bt = paged(cuda, 345, lens, 16, 2, 128, BF)
+    q, kl, st = torch.randn(2, 8, 128, generator=gen, device=cuda).to(BF), i32(lens), i32([0, 1, 2])
+    out, lse = torch.empty_like(q), torch.empty(2, 8, device=cuda)
+    calls = [lambda: b200decode.decode(q, k, v, kl, bt, out=out, lse=lse),
+             lambda: b200decode.cross_attention(q, k, v, kl, bt, query_starts=st, out=out, lse=lse),
+             lambda: b200decode.cross_attention(q, k, v, kl, bt, out=out, lse=lse),
+             lambda: b200decode.decode_shared_prefix(q, k, v, kl[:1], bt[:1], kl, bt, out=out, lse=lse)]
+    for call in calls:
+        want = [x.clone() for x in call()]
+        torch.cuda.synchronize()
+        got = []
+
+        def work():
+            try:
+                got.extend(x.clone() for x in call())
+            except Exception as e:   # noqa: BLE001
+                got.append(e)
+
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert len(got) == 2, got
+        assert all(torch.equal(x, y) for x, y in zip(got, want))

@@ -44,11 +44,16 @@ class DecodeWorkspace:
     enqueued on different streams never share partials.  A workspace is
     allocated, and re-allocated when it grows, on the stream it serves, so
     torch's caching allocator recycles the old buffer only in that stream's
-    order (after the last decode that read it)."""
+    order (after the last decode that read it).
+
+    Host threads may share a workspace (on one stream): a call holds `lock`
+    while it binds the buffer and enqueues its launches, which hand partials to
+    each other through it."""
 
     def __init__(self, device: torch.device, nbytes: int = 0, stream=None):
         self.device = torch.device(device)
         self.stream = stream
+        self.lock = threading.RLock()
         self.captured = False   # a CUDA graph holds this buffer's address
         self.buf = self._alloc(max(nbytes, 1 << 20))
 
@@ -58,6 +63,7 @@ class DecodeWorkspace:
         graph's pool, its header zeroed by a node of the graph."""
         ws = cls.__new__(cls)
         ws.device, ws.stream, ws.captured = torch.device(device), None, True
+        ws.lock = threading.RLock()
         ws.buf = torch.empty(max(nbytes, _lib.B2D_WORKSPACE_HEADER_BYTES), dtype=torch.uint8, device=device)
         ws.buf[:_lib.B2D_WORKSPACE_HEADER_BYTES].zero_()
         return ws
@@ -232,10 +238,11 @@ def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     ws = workspace or _default_ws(q.device)
     need = C.c_size_t(0)
     _check(lib.b2d_gqa_workspace_bytes(C.byref(a), C.byref(need)), "b2d_gqa_workspace_bytes")
-    ws.ensure(need.value)
-    a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
     stream = torch.cuda.current_stream(q.device).cuda_stream
-    _check(lib.b2d_decode_gqa(C.byref(a), C.c_void_p(stream)), "b2d_decode_gqa")
+    with ws.lock:
+        ws.ensure(need.value)
+        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+        _check(lib.b2d_decode_gqa(C.byref(a), C.c_void_p(stream)), "b2d_decode_gqa")
     return out, lse
 
 
@@ -273,16 +280,18 @@ class GqaDecoder:
         need = C.c_size_t(0)
         _check(self._lib.b2d_gqa_workspace_bytes(C.byref(self._args), C.byref(need)),
                "b2d_gqa_workspace_bytes")
-        self.ws.ensure(need.value)
-        self._ws_buf = self.ws.buf   # pin the buffer this plan points at
-        self._args.workspace, self._args.workspace_bytes = self.ws.ptr, self.ws.nbytes
+        with self.ws.lock:
+            self.ws.ensure(need.value)
+            self._ws_buf = self.ws.buf   # pin the buffer this plan points at
+            self._args.workspace, self._args.workspace_bytes = self.ws.ptr, self.ws.nbytes
         self._argp = C.byref(self._args)
         self._fn = self._lib.b2d_decode_gqa
         self.device = q.device
         self._graph = None
 
     def run(self):
-        rc = self._fn(self._argp, C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream))
+        with self.ws.lock:
+            rc = self._fn(self._argp, C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream))
         if rc:
             raise B2DError(rc, "b2d_decode_gqa")
         return self.out, self.lse
@@ -365,10 +374,11 @@ def decode_mla(q: torch.Tensor, kv_cache: torch.Tensor, cache_seqlens: torch.Ten
     ws = workspace or _default_ws(q.device)
     need = C.c_size_t(0)
     _check(lib.b2d_mla_workspace_bytes(C.byref(a), C.byref(need)), "b2d_mla_workspace_bytes")
-    ws.ensure(need.value)
-    a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
     stream = torch.cuda.current_stream(q.device).cuda_stream
-    _check(lib.b2d_decode_mla(C.byref(a), C.c_void_p(stream)), "b2d_decode_mla")
+    with ws.lock:
+        ws.ensure(need.value)
+        a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
+        _check(lib.b2d_decode_mla(C.byref(a), C.c_void_p(stream)), "b2d_decode_mla")
     return out, lse
 
 

@@ -112,12 +112,13 @@ def plan_append(cache_seqlens: torch.Tensor, block_table: torch.Tensor, free_pag
         _check_out(where, "free_count_out", free_count_out, 1, torch.int32)
     with _on(index):
         ws = _workspace(workspace, index, lambda: _HEADER)
-        a = _lib.PlanAppendArgs(cache_seqlens.data_ptr(), _ptr(new_tokens), block_table.data_ptr(),
-                                block_table.stride(0), free_pages.data_ptr(), free_count.data_ptr(),
-                                slot_mapping.data_ptr(), query_starts.data_ptr(), seqlens_out.data_ptr(),
-                                free_count_out.data_ptr(), bsz, block_table.shape[1], page_size, max_tokens,
-                                free_pages.shape[0], 0, ws.ptr, ws.nbytes)
-        rc = _lib.load().b2d_plan_append(C.byref(a), _stream(index))
+        with ws.lock:
+            a = _lib.PlanAppendArgs(cache_seqlens.data_ptr(), _ptr(new_tokens), block_table.data_ptr(),
+                                    block_table.stride(0), free_pages.data_ptr(), free_count.data_ptr(),
+                                    slot_mapping.data_ptr(), query_starts.data_ptr(), seqlens_out.data_ptr(),
+                                    free_count_out.data_ptr(), bsz, block_table.shape[1], page_size, max_tokens,
+                                    free_pages.shape[0], 0, ws.ptr, ws.nbytes)
+            rc = _lib.load().b2d_plan_append(C.byref(a), _stream(index))
     if rc:
         raise B2DError(rc, "b2d_plan_append")
     return AppendPlan(slot_mapping, query_starts, seqlens_out, free_count_out)
@@ -154,11 +155,12 @@ def release_pages(cache_seqlens: torch.Tensor, block_table: torch.Tensor, finish
         _check_out(where, "free_count_out", free_count_out, 1, torch.int32)
     with _on(index):
         ws = _workspace(workspace, index, lambda: _HEADER)
-        a = _lib.ReleaseArgs(cache_seqlens.data_ptr(), finished.data_ptr(), block_table.data_ptr(),
-                             block_table.stride(0), free_pages.data_ptr(), free_count.data_ptr(),
-                             seqlens_out.data_ptr(), free_count_out.data_ptr(), bsz, block_table.shape[1],
-                             page_size, free_pages.shape[0], ws.ptr, ws.nbytes)
-        rc = _lib.load().b2d_release_pages(C.byref(a), _stream(index))
+        with ws.lock:
+            a = _lib.ReleaseArgs(cache_seqlens.data_ptr(), finished.data_ptr(), block_table.data_ptr(),
+                                 block_table.stride(0), free_pages.data_ptr(), free_count.data_ptr(),
+                                 seqlens_out.data_ptr(), free_count_out.data_ptr(), bsz, block_table.shape[1],
+                                 page_size, free_pages.shape[0], ws.ptr, ws.nbytes)
+            rc = _lib.load().b2d_release_pages(C.byref(a), _stream(index))
     if rc:
         raise B2DError(rc, "b2d_release_pages")
     return seqlens_out, free_count_out

@@ -88,13 +88,15 @@ def _call(fn, name: str, a, own, workspace: Optional[DecodeWorkspace], index: in
         _check(query(C.byref(a), C.byref(n)), name)
         return n.value
     ws = _workspace(workspace, index, need)
-    buf = ws.buf
-    own.workspace, own.workspace_bytes = buf.data_ptr(), buf.numel()
-    rc = fn(C.byref(a), _stream(index))
-    if rc == _lib.B2D_ERR_WORKSPACE:
-        ws.ensure(need())
-        own.workspace, own.workspace_bytes = ws.ptr, ws.nbytes
+    # (one call at a time: its launches hand partials to each other in the workspace)
+    with ws.lock:
+        buf = ws.buf
+        own.workspace, own.workspace_bytes = buf.data_ptr(), buf.numel()
         rc = fn(C.byref(a), _stream(index))
+        if rc == _lib.B2D_ERR_WORKSPACE:
+            ws.ensure(need())
+            own.workspace, own.workspace_bytes = ws.ptr, ws.nbytes
+            rc = fn(C.byref(a), _stream(index))
     if rc:
         raise B2DError(rc, name)
 

@@ -153,3 +153,43 @@ def test_first_call_of_a_host_thread(cuda):
         torch.cuda.synchronize()
         assert len(got) == 2, got
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+def test_host_threads_on_one_stream(cuda):
+    """Threads that share a stream share its default workspace: the launches of
+    one call are not mixed with another's."""
+    P, hkv, hq, d = 16, 2, 8, 128
+    lens = [900, 700, 300, 40, 500]
+    gen, k, v, _, _, bt = paged(cuda, 350, lens, P, hkv, d, BF)
+    kl = i32(lens)
+    qs = [torch.randn(40, hq, d, generator=gen, device=cuda).to(BF) for _ in range(4)]
+    own, obt = i32([300 + i for i in range(40)]), bt[1:2].repeat(40, 1)
+    pool = torch.arange(1000, dtype=torch.int32, device=cuda)
+    calls = [
+        lambda: b200decode.decode_shared_prefix(qs[0], k, v, kl[:1], bt[:1], own, obt),
+        lambda: b200decode.decode_shared_prefix(qs[1], k, v, kl[2:3], bt[2:3], own, obt, softmax_scale=0.2),
+        lambda: b200decode.cross_attention(qs[2], k, v, kl, bt, query_starts=i32([0, 9, 20, 21, 30, 40])),
+        lambda: b200decode.decode(qs[3][:5], k, v, kl, bt),
+        lambda: b200decode.plan_append(kl, bt.clone(), pool, i32([1000]), P)[:3],
+    ]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    wrong, ready = [], threading.Barrier(len(calls))
+
+    def work(i):
+        try:
+            ready.wait()
+            got = [calls[i]() for _ in range(60)]
+            torch.cuda.synchronize()
+            for g in got:
+                if not all(torch.equal(x, y) for x, y in zip(g, want[i])):
+                    wrong.append(i)
+        except Exception as e:   # noqa: BLE001
+            wrong.append((i, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    b200decode.check_device_status()

@@ -1,0 +1,61 @@
+"""What calls do with a workspace on the host: one call at a time binds it and
+enqueues (no GPU needed: the library's entry is a stand-in)."""
+import threading
+import time
+
+import pytest
+import torch
+
+from b200decode import _lib, ragged
+from b200decode.api import DecodeWorkspace
+
+
+@pytest.fixture
+def host(monkeypatch):
+    monkeypatch.setattr(ragged, "_stream", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return torch.device("cpu")
+
+
+class Entry:
+    """A library entry that enqueues two launches; says "too small" below `needs` bytes."""
+
+    def __init__(self, ws, needs):
+        self.ws, self.needs, self.log = ws, needs, []
+
+    def __call__(self, ref, stream):
+        args = ref._obj
+        if args.workspace_bytes < self.needs[args.batch]:
+            time.sleep(0.002)
+            return _lib.B2D_ERR_WORKSPACE
+        for launch in range(2):
+            self.log.append((args.batch, launch, args.workspace == self.ws.buf.data_ptr()))
+            time.sleep(0.002)
+        return 0
+
+    def query(self, ref, n):
+        n._obj.value = self.needs[ref._obj.batch]
+        return 0
+
+
+def test_one_call_at_a_time_in_a_workspace(host):
+    """Threads that share a workspace, some of which make it grow: the launches
+    of a call stand together, and each call's go to the buffer of the time."""
+    ws = DecodeWorkspace(host)
+    entry = Entry(ws, {i: (1 << 20) * (1 + i) for i in range(6)})
+
+    def work(i):
+        for _ in range(4):
+            a = _lib.GqaArgs()
+            a.batch = i
+            ragged._call(entry, "entry", a, a, ws, -1, entry.query)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(entry.log) == 48
+    for first, second in zip(entry.log[::2], entry.log[1::2]):
+        assert first[0] == second[0] and (first[1], second[1]) == (0, 1)
+        assert first[2] and second[2]

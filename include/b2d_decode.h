@@ -309,7 +309,8 @@ int b2d_cross_attention(const b2d_cross_args* args, void* stream);
  *              [group_starts[g], group_starts[g + 1]); sequences outside
  *              every group have no prefix.  NULL: one group with all.
  * Either part may be empty; both: out = 0, lse = -inf.  out overlaps no input.
- * num_groups <= 4096.
+ * num_groups <= 4096.  Sizes as b2d_decode_gqa takes them: it runs the own
+ * tokens, and B2D_ERR_UNSUPPORTED for own is the answer here too.
  */
 typedef struct b2d_shared_prefix_args {
   b2d_gqa_args own;

@@ -14,7 +14,7 @@ B2D_KV_STRIDED, B2D_KV_VLLM = 0, 1
 B2D_BF16, B2D_FP16, B2D_FP8_E4M3, B2D_FP32 = 0, 1, 2, 3
 B2D_FLAG_SKIP_COMBINE, B2D_FLAG_COMBINE_ONLY, B2D_FLAG_TEST_NO_LOADS = 1, 2, 4
 B2D_WORKSPACE_HEADER_BYTES = 65792
-B2D_ERR_WORKSPACE, B2D_ERR_DEVICE_CAPACITY = -4, -9
+B2D_ERR_UNSUPPORTED, B2D_ERR_WORKSPACE, B2D_ERR_DEVICE_CAPACITY = -2, -4, -9
 
 EXPORTED = (
     "b2d_gqa_workspace_bytes",

@@ -150,7 +150,8 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     q: ragged [T, Hq, D] with query_starts int32 [B + 1] (request b owns
     tokens query_starts[b] .. query_starts[b + 1] - 1, ascending), or dense
     [B, Tq, Hq, D], or [B, Hq, D] for one token each, which is decode()'s
-    kernel.  Caches, scales and layouts as in decode(); kv_lens int32 [B],
+    kernel where that takes the sizes.  Up to 32 query heads per KV head.
+    Caches, scales and layouts as in decode(); kv_lens int32 [B],
     block_table int32 [B, max_pages].  softmax_scale defaults to 1/sqrt(D).
     Returns out (shape of q) and lse (shape of q without D, fp32, natural
     log).  A request without states gives out = 0, lse = -inf; ragged tokens
@@ -211,19 +212,23 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         return out, lse
     lib = _lib.load()
     with _on(index):
-        # One token each is decode(); head_dim 192 outside what that is built for stays here.
-        if length == 1 and not flags and (d != 192 or (page % 16 == 0 and k_cache.dtype is q.dtype)):
-            ws = workspace
-            if ws is not None or torch.cuda.is_current_stream_capturing():
-                g = _gqa_args(q3, k_cache, v_cache, kv_lens, block_table, softmax_scale, k_scale, v_scale, out3,
-                              lse2, kv_layout, num_ctas)
-                need = C.c_size_t(0)
-                _check(lib.b2d_gqa_workspace_bytes(C.byref(g), C.byref(need)), "b2d_gqa_workspace_bytes")
-                ws = _workspace(workspace, index, lambda: need.value)
-            decode(q3, k_cache, v_cache, kv_lens, block_table, softmax_scale, k_scale=k_scale, v_scale=v_scale,
-                   out=out3, lse=lse2, kv_layout=kv_layout, num_ctas=num_ctas, workspace=ws,
-                   wait_limit_us=wait_limit_us)
-            return out, lse
+        # One token each is decode(), for the sizes that it takes (it says so before it enqueues anything).
+        if length == 1 and not flags:
+            try:
+                ws = workspace
+                if ws is not None or torch.cuda.is_current_stream_capturing():
+                    g = _gqa_args(q3, k_cache, v_cache, kv_lens, block_table, softmax_scale, k_scale, v_scale, out3,
+                                  lse2, kv_layout, num_ctas)
+                    need = C.c_size_t(0)
+                    _check(lib.b2d_gqa_workspace_bytes(C.byref(g), C.byref(need)), "b2d_gqa_workspace_bytes")
+                    ws = _workspace(workspace, index, lambda: need.value)
+                decode(q3, k_cache, v_cache, kv_lens, block_table, softmax_scale, k_scale=k_scale, v_scale=v_scale,
+                       out=out3, lse=lse2, kv_layout=kv_layout, num_ctas=num_ctas, workspace=ws,
+                       wait_limit_us=wait_limit_us)
+                return out, lse
+            except B2DError as e:
+                if e.code != _lib.B2D_ERR_UNSUPPORTED:
+                    raise
         fp8 = k_cache.dtype is torch.float8_e4m3fn
         qs, so = q3.stride(), out3.stride()
         a = _lib.CrossArgs(
@@ -257,8 +262,13 @@ def decode_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     as pages of the same caches.  group_starts int32 [G + 1], ascending: group g
     holds sequences group_starts[g] .. group_starts[g + 1] - 1 (sequences
     outside every group have no prefix); None: one group with the whole batch.
-    The rest as in decode().  Out is computed in fp32 over both parts and
-    rounded once; it must not overlap q.
+    The rest as in decode(), whose kernels take the own tokens and whose limits
+    hold here too: the query heads of a KV head split into at most 8 equal
+    parts of at most 16 (8 at head_dim 192 and 256); with pages that are no
+    multiples of 16, or e4m3 at head_dim 64, they are at most 8, or 16 if even;
+    head_dim 192 takes 16-bit caches in pages of multiples of 16 alone.
+    Out is computed in fp32 over both parts and rounded once;
+    it must not overlap q.
 
     With a table whose rows begin with a common prefix of n full pages, pass
     prefix_block_table = table[:1, :n], block_table = table[:, n:] and the

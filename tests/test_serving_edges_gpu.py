@@ -193,3 +193,41 @@ def test_host_threads_on_one_stream(cuda):
         t.join()
     assert not wrong
     b200decode.check_device_status()
+
+
+# ---------------------------------------------------------------- sizes
+
+ONE_TOKEN = [
+    # Hq, Hkv, D, P, q dtype, cache dtype: sizes that decode()'s kernels do not take, and two that they do
+    (9, 1, 128, 5, BF, BF), (32, 1, 128, 8, BF, BF), (11, 1, 256, 16, BF, BF), (17, 1, 128, 16, HF, HF),
+    (62, 2, 128, 16, BF, BF), (32, 1, 64, 16, BF, F8), (11, 1, 64, 16, HF, F8), (26, 1, 256, 16, BF, F8),
+    (8, 2, 192, 5, BF, BF), (8, 2, 192, 16, HF, F8), (16, 1, 128, 16, BF, BF), (8, 2, 192, 16, BF, BF),
+]
+
+
+@pytest.mark.parametrize("case", range(len(ONE_TOKEN)))
+@pytest.mark.parametrize("form", ["BHD", "B1HD", "workspace", "captured"])
+def test_cross_attention_of_one_token_takes_every_group(cuda, case, form):
+    """Up to 32 query heads per KV head at every head_dim, page size and cache
+    type, as with several tokens."""
+    hq, hkv, d, P, qd, kv = ONE_TOKEN[case]
+    lens = [1, 300, 0, 77]
+    gen, k, v, ks, vs, bt = paged(cuda, 300 + case, lens, P, hkv, d, kv)
+    q = torch.randn(4, hq, d, generator=gen, device=cuda).to(qd)
+    kl, kw = i32(lens), dict(k_scale=ks, v_scale=vs)
+    if form == "workspace":
+        kw["workspace"] = b200decode.DecodeWorkspace(cuda, 64 << 20)
+    call = lambda: b200decode.cross_attention(q[:, None] if form == "B1HD" else q, k, v, kl, bt, **kw)  # noqa: E731
+    out, lse = call()
+    if form == "captured":
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out, lse = call()
+        g.replay()
+    torch.cuda.synchronize()
+    b200decode.check_device_status(kw.get("workspace"))
+    for b, n in enumerate(lens):
+        r = attend(q[b:b + 1].double(), gather(k, ks, bt[b], n, "NHD"), gather(v, vs, bt[b], n, "NHD"), d ** -0.5, kv)
+        check(out.reshape(4, hq, d)[b:b + 1], r[0], r[2], u_of(qd), "out")
+        check_lse(lse.reshape(4, hq)[b:b + 1], r[1], r[3])

@@ -53,7 +53,7 @@ enum b2d_status {
   B2D_ERR_WORKSPACE = -4,        /* workspace missing or too small          */
   B2D_ERR_CUDA = -5,             /* a CUDA runtime/driver call failed       */
   B2D_ERR_DEVICE_TIMEOUT = -6,   /* a kernel gave up waiting (status word)  */
-  B2D_ERR_DEVICE_BOUNDS = -7,    /* a kernel saw a page id out of range     */
+  B2D_ERR_DEVICE_BOUNDS = -7,    /* page id out of range, starts descending */
   B2D_ERR_TOO_LARGE = -8,        /* a size beyond the documented maximum    */
   B2D_ERR_DEVICE_CAPACITY = -9   /* pages, table or slots too few (status)  */
 };
@@ -257,7 +257,9 @@ int b2d_append_kv(const b2d_append_args* args, void* stream);
  *              max_pages_per_seq]
  *   lse        [num_tokens, num_q_heads] fp32 (may be NULL)
  * A request without states yields out = 0 and lse = -inf; tokens behind
- * query_starts[num_groups] are left as they were.  out overlaps no input.
+ * query_starts[num_groups] are left as they were.  Starts that descend: out and
+ * lse are left as they were and the status word reports B2D_ERR_DEVICE_BOUNDS.
+ * out overlaps no input.
  * head_dim 64, 128, 192 and 256, group (num_q_heads / num_kv_heads) <= 32.
  */
 typedef struct b2d_cross_args {
@@ -307,7 +309,8 @@ int b2d_cross_attention(const b2d_cross_args* args, void* stream);
  *              prefix_max_pages]: pages in the same caches
  *   group_starts int32 [num_groups + 1]: group g holds sequences
  *              [group_starts[g], group_starts[g + 1]); sequences outside
- *              every group have no prefix.  NULL: one group with all.
+ *              every group have no prefix.  NULL: one group with all.  Starts
+ *              that descend: as those of b2d_cross_args.
  * Either part may be empty; both: out = 0, lse = -inf.  out overlaps no input.
  * num_groups <= 4096.  Sizes as b2d_decode_gqa takes them: it runs the own
  * tokens, and B2D_ERR_UNSUPPORTED for own is the answer here too.
@@ -423,7 +426,8 @@ int b2d_release_pages(const b2d_release_args* args, void* stream);
 
 /*
  * Reads (and clears, when clear != 0) the device status word that kernels
- * set when an in-kernel wait ran out of time or a page id was out of range.
+ * set when an in-kernel wait ran out of time, a page id was out of range, group
+ * starts descended or a step did not fit.
  * Synchronises `stream`.  Returns 0 or the matching negative b2d_status.
  */
 int b2d_check_device_status(void* workspace, int clear, void* stream);

@@ -156,6 +156,8 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Returns out (shape of q) and lse (shape of q without D, fp32, natural
     log).  A request without states gives out = 0, lse = -inf; ragged tokens
     behind query_starts[B] are left as they were.  out must not overlap q.
+    query_starts that descend are reported (check_device_status(),
+    B2D_ERR_DEVICE_BOUNDS) and nothing is written.
 
     Captured into a CUDA graph without `workspace`, a call keeps its scratch
     in the graph's memory pool; check_device_status() reads the status only of
@@ -261,7 +263,8 @@ def decode_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     int32 [B] and block_table int32 [B, max_pages] the sequences' own tokens, all
     as pages of the same caches.  group_starts int32 [G + 1], ascending: group g
     holds sequences group_starts[g] .. group_starts[g + 1] - 1 (sequences
-    outside every group have no prefix); None: one group with the whole batch.
+    outside every group have no prefix; starts that descend are reported, as in
+    cross_attention()); None: one group with the whole batch.
     The rest as in decode(), whose kernels take the own tokens and whose limits
     hold here too: the query heads of a KV head split into at most 8 equal
     parts of at most 16 (8 at head_dim 192 and 256); with pages that are no

@@ -13,7 +13,7 @@ extern "C" const char* b2d_error_string(int status) {
     case B2D_ERR_WORKSPACE: return "workspace missing or too small";
     case B2D_ERR_CUDA: return "CUDA runtime or driver call failed";
     case B2D_ERR_DEVICE_TIMEOUT: return "a kernel gave up waiting on a pipeline barrier";
-    case B2D_ERR_DEVICE_BOUNDS: return "a block-table page id was out of range";
+    case B2D_ERR_DEVICE_BOUNDS: return "a page id was out of range, or group starts descend";
     case B2D_ERR_TOO_LARGE: return "size beyond the supported maximum";
     case B2D_ERR_DEVICE_CAPACITY:
       return "a step found too few free pages, block-table columns or token slots";

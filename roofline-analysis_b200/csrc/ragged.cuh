@@ -114,17 +114,22 @@ __host__ __device__ constexpr size_t ragged_table_bytes(int groups) {
   return ((size_t)groups + 1 + 32 + (groups <= kCachedGroups ? 3 * (size_t)groups : 0)) * 4;
 }
 
-// Fills the table (block-wide scan; ends with __syncthreads).
-__device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* table) {
+// Fills the table (block-wide scan; ends with __syncthreads).  False, with a
+// table of no work: the starts descend somewhere.  Tokens would then belong to
+// several groups, whose rows race, and the work line could pass 32 bits (the
+// host's bound counts every token once).
+__device__ __forceinline__ bool ragged_table(const RaggedParams& p, int32_t* table) {
   int32_t* warp_tmp = table + p.G + 1;
   int32_t* cache = p.G <= kCachedGroups ? warp_tmp + 32 : nullptr;
   const int tid = threadIdx.x, nth = blockDim.x;
   const int lane = tid & 31, warp = tid >> 5, nwarps = nth >> 5;
   int carry = 0;
+  bool descends = false;
   for (int base = 0; base < p.G; base += nth) {
     const int g = base + tid;
     int n = 0;
     if (g < p.G) {
+      descends = descends || (p.starts != nullptr && __ldg(p.starts + g + 1) < __ldg(p.starts + g));
       const int2 tok = ragged_tokens(p, g);
       const int len = ragged_kv_len(p, g), nch = (len + p.CH - 1) / p.CH;
       n = nch > 0 ? ragged_items(p, tok.y) * (nch + kItemCost) : 0;
@@ -157,8 +162,11 @@ __device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* tab
     __syncthreads();
     carry += total;
   }
-  if (tid == 0) table[p.G] = carry;
+  descends = __syncthreads_or(descends);
+  if (tid == 0) table[p.G] = descends ? 0 : carry;
+  if (descends && tid == 0 && blockIdx.x == 0) record_status(p.status, kStatusBounds);
   __syncthreads();
+  return !descends;
 }
 
 // A piece of an item, inside one range: chunks [c0, c1) of nch.  Part s (0 or

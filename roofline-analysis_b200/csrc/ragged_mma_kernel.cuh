@@ -61,8 +61,7 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
 
   griddep_wait();
   griddep_launch();
-  ragged_table(p, table);
-  ragged_rows_without_keys<D, QT>(p);
+  if (ragged_table(p, table)) ragged_rows_without_keys<D, QT>(p);
   const int W = table[p.G];
   const int ctas = W < (int)gridDim.x ? W : (int)gridDim.x;
   if (tid == 0) ragged_note_cut(p, blockIdx.x, nullptr, W, ctas);   // nothing yet

@@ -231,3 +231,29 @@ def test_cross_attention_of_one_token_takes_every_group(cuda, case, form):
         r = attend(q[b:b + 1].double(), gather(k, ks, bt[b], n, "NHD"), gather(v, vs, bt[b], n, "NHD"), d ** -0.5, kv)
         check(out.reshape(4, hq, d)[b:b + 1], r[0], r[2], u_of(qd), "out")
         check_lse(lse.reshape(4, hq)[b:b + 1], r[1], r[3])
+
+
+@pytest.mark.parametrize("P", [16, 5])
+@pytest.mark.parametrize("starts", [[0, 12, 5, 20], [3, 1, 1, 20], [0, 20, 20, 19]])
+def test_descending_starts_are_reported(cuda, P, starts):
+    """Starts that descend would give tokens to two groups: nothing is written,
+    and the status says so."""
+    gen, k, v, _, _, bt = paged(cuda, 310, [96, 64, 40], P, 2, 64, BF)
+    q = torch.randn(20, 4, 64, generator=gen, device=cuda).to(BF)
+    kl, st = i32([96, 64, 40]), i32(starts)
+    ws = b200decode.DecodeWorkspace(cuda, 64 << 20)
+    own, obt = i32([3] * 20), bt[:1].repeat(20, 1)
+    for call in (lambda **kw: b200decode.cross_attention(q, k, v, kl, bt, workspace=ws, **kw),
+                 lambda **kw: b200decode.decode_shared_prefix(q, k, v, kl, bt, own, obt, workspace=ws,
+                                                              group_starts=kw.pop("query_starts"), **kw)):
+        out, lse = torch.full_like(q, 7.0), torch.full((20, 4), 7.0, device=cuda)
+        call(query_starts=st, out=out, lse=lse)
+        torch.cuda.synchronize()
+        with pytest.raises(b200decode.B2DError) as e:
+            b200decode.check_device_status(ws)
+        assert e.value.code == -7
+        assert (out == 7).all() and (lse == 7).all()
+        a = call(query_starts=i32([0, 12, 15, 20]))
+        b200decode.check_device_status(ws)
+        b = call(query_starts=i32([0, 12, 15, 20]))
+        assert torch.equal(a[0], b[0]) and torch.isfinite(a[0]).all()

@@ -11,6 +11,7 @@ flashmla_kernel.py:45-46) or B2DError (a RuntimeError) for library codes.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 from typing import Optional, Tuple
@@ -21,6 +22,7 @@ from . import _lib
 
 _DT = {torch.bfloat16: _lib.B2D_BF16, torch.float16: _lib.B2D_FP16,
        torch.float8_e4m3fn: _lib.B2D_FP8_E4M3}
+_STATUS_BYTES = 4   # the status word, first of a workspace's header
 
 
 class B2DError(RuntimeError):
@@ -68,10 +70,11 @@ class DecodeWorkspace:
         ws.buf[:_lib.B2D_WORKSPACE_HEADER_BYTES].zero_()
         return ws
 
+    def _on_stream(self):
+        return contextlib.nullcontext() if self.stream is None else torch.cuda.stream(self.stream)
+
     def _alloc(self, n: int) -> torch.Tensor:
-        if self.stream is None:
-            return torch.zeros(n, dtype=torch.uint8, device=self.device)
-        with torch.cuda.stream(self.stream):
+        with self._on_stream():
             return torch.zeros(n, dtype=torch.uint8, device=self.device)
 
     def ensure(self, nbytes: int) -> "DecodeWorkspace":
@@ -79,7 +82,11 @@ class DecodeWorkspace:
             if self.captured:
                 raise ValueError(f"a workspace that a CUDA graph holds cannot grow (it has {self.buf.numel()} "
                                  f"bytes, {nbytes} are needed): size it before the capture")
-            self.buf = self._alloc(int(nbytes * 1.25) + 4096)
+            old, self.buf = self.buf, self._alloc(int(nbytes * 1.25) + 4096)
+            # a status that was recorded and not read stays (a graph under capture would copy it at each replay)
+            if not (old.is_cuda and torch.cuda.is_current_stream_capturing()):
+                with self._on_stream():
+                    self.buf[:_STATUS_BYTES].copy_(old[:_STATUS_BYTES])
         return self
 
     @property

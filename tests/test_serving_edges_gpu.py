@@ -257,3 +257,19 @@ def test_descending_starts_are_reported(cuda, P, starts):
         b200decode.check_device_status(ws)
         b = call(query_starts=i32([0, 12, 15, 20]))
         assert torch.equal(a[0], b[0]) and torch.isfinite(a[0]).all()
+
+
+def test_status_of_a_call_outlives_growth_by_the_next(cuda):
+    gen, k, v, _, _, bt = paged(cuda, 315, [100, 50], 16, 2, 64, BF)
+    q = torch.randn(70, 4, 64, generator=gen, device=cuda).to(BF)
+    st, kl, bad = i32([0, 40, 70]), i32([100, 50]), bt.clone()
+    bad[0, 2] = -1
+    ws = b200decode.DecodeWorkspace(cuda)
+    b200decode.cross_attention(q, k, v, kl, bad, query_starts=st, workspace=ws, num_ctas=2)
+    size = ws.nbytes
+    b200decode.cross_attention(q, k, v, kl, bt, query_starts=st, workspace=ws, num_ctas=300)
+    assert ws.nbytes > size
+    with pytest.raises(b200decode.B2DError) as e:
+        b200decode.check_device_status(ws)
+    assert e.value.code == -7
+    b200decode.check_device_status(ws)

@@ -59,3 +59,14 @@ def test_one_call_at_a_time_in_a_workspace(host):
     for first, second in zip(entry.log[::2], entry.log[1::2]):
         assert first[0] == second[0] and (first[1], second[1]) == (0, 1)
         assert first[2] and second[2]
+
+
+def test_status_outlives_growth(host):
+    """A recorded status that nobody has read yet moves to the larger buffer;
+    the arrival counters behind it start at zero."""
+    ws = DecodeWorkspace(host)
+    ws.buf[:8] = torch.tensor([2, 0, 0, 0, 9, 9, 9, 9], dtype=torch.uint8)
+    old = ws.nbytes
+    ws.ensure(old + 1)
+    assert ws.nbytes > old
+    assert ws.buf[:8].tolist() == [2, 0, 0, 0, 0, 0, 0, 0] and not ws.buf[8:].any()

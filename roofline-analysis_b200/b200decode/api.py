@@ -48,6 +48,11 @@ class DecodeWorkspace:
     torch's caching allocator recycles the old buffer only in that stream's
     order (after the last decode that read it).
 
+    A workspace that was given to a serving call under capture refuses to grow
+    from then on (also after the graph is gone, which it does not learn): take
+    one for each set of graphs.  decode() and decode_mla() under capture keep the
+    buffer of the time alive instead, and the workspace may grow.
+
     Host threads may share a workspace (on one stream): a call holds `lock`
     while it binds the buffer and enqueues its launches, which hand partials to
     each other through it."""
@@ -56,7 +61,8 @@ class DecodeWorkspace:
         self.device = torch.device(device)
         self.stream = stream
         self.lock = threading.RLock()
-        self.captured = False   # a CUDA graph holds this buffer's address
+        self.captured = False   # a CUDA graph holds this buffer's address: it may not grow
+        self.held: list = []    # buffers that graphs of decode() calls hold, kept as long as the workspace
         self.buf = self._alloc(max(nbytes, 1 << 20))
 
     @classmethod
@@ -65,10 +71,16 @@ class DecodeWorkspace:
         graph's pool, its header zeroed by a node of the graph."""
         ws = cls.__new__(cls)
         ws.device, ws.stream, ws.captured = torch.device(device), None, True
-        ws.lock = threading.RLock()
+        ws.lock, ws.held = threading.RLock(), []
         ws.buf = torch.empty(max(nbytes, _lib.B2D_WORKSPACE_HEADER_BYTES), dtype=torch.uint8, device=device)
         ws.buf[:_lib.B2D_WORKSPACE_HEADER_BYTES].zero_()
         return ws
+
+    def hold(self) -> None:
+        """Keeps the present buffer for a graph under capture: the workspace may
+        grow later, the graph goes on with this one."""
+        if not any(b is self.buf for b in self.held):
+            self.held.append(self.buf)
 
     def _on_stream(self):
         return contextlib.nullcontext() if self.stream is None else torch.cuda.stream(self.stream)
@@ -248,6 +260,8 @@ def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     stream = torch.cuda.current_stream(q.device).cuda_stream
     with ws.lock:
         ws.ensure(need.value)
+        if torch.cuda.is_current_stream_capturing():
+            ws.hold()
         a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
         _check(lib.b2d_decode_gqa(C.byref(a), C.c_void_p(stream)), "b2d_decode_gqa")
     return out, lse
@@ -384,6 +398,8 @@ def decode_mla(q: torch.Tensor, kv_cache: torch.Tensor, cache_seqlens: torch.Ten
     stream = torch.cuda.current_stream(q.device).cuda_stream
     with ws.lock:
         ws.ensure(need.value)
+        if torch.cuda.is_current_stream_capturing():
+            ws.hold()
         a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
         _check(lib.b2d_decode_mla(C.byref(a), C.c_void_p(stream)), "b2d_decode_mla")
     return out, lse
@@ -467,5 +483,6 @@ def check_device_status(workspace: Optional[DecodeWorkspace] = None, device=None
     stream = torch.cuda.current_stream(device).cuda_stream
     torch.cuda.synchronize(device)
     for ws in spaces:
-        _check(lib.b2d_check_device_status(C.c_void_p(ws.ptr), int(clear), C.c_void_p(stream)),
-               "device status")
+        for buf in (ws.buf, *(b for b in ws.held if b is not ws.buf)):
+            _check(lib.b2d_check_device_status(C.c_void_p(buf.data_ptr()), int(clear), C.c_void_p(stream)),
+                   "device status")

@@ -273,3 +273,27 @@ def test_status_of_a_call_outlives_growth_by_the_next(cuda):
         b200decode.check_device_status(ws)
     assert e.value.code == -7
     b200decode.check_device_status(ws)
+
+
+def test_buffer_of_a_captured_decode_outlives_growth(cuda):
+    """A graph that holds a workspace's buffer replays into memory that is its
+    own, also after a later call made the workspace grow."""
+    gen, k, v, _, _, bt = paged(cuda, 360, [5000, 3000], 16, 2, 128, BF)
+    q, kl = torch.randn(2, 8, 128, generator=gen, device=cuda).to(BF), i32([5000, 3000])
+    ws = b200decode.DecodeWorkspace(cuda)
+    want = b200decode.decode(q, k, v, kl, bt, workspace=ws)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = b200decode.decode(q, k, v, kl, bt, workspace=ws)
+    old = ws.buf.data_ptr()
+    many = torch.randn(300, 8, 128, generator=gen, device=cuda).to(BF)
+    b200decode.cross_attention(many, k, v, kl, bt, query_starts=i32([0, 100, 300]), workspace=ws, num_ctas=600)
+    assert ws.buf.data_ptr() != old
+    fill = [torch.full((1 << 20,), 77, dtype=torch.uint8, device=cuda) for _ in range(8)]
+    assert all(f.data_ptr() != old for f in fill)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert all((f == 77).all() for f in fill)
+    b200decode.check_device_status(ws)

@@ -70,3 +70,17 @@ def test_status_outlives_growth(host):
     ws.ensure(old + 1)
     assert ws.nbytes > old
     assert ws.buf[:8].tolist() == [2, 0, 0, 0, 0, 0, 0, 0] and not ws.buf[8:].any()
+
+
+def test_held_buffer_outlives_growth(host):
+    """hold() keeps the buffer that a captured decode() was given; a workspace
+    that must not grow still refuses to."""
+    ws = DecodeWorkspace(host)
+    held = ws.buf
+    ws.hold()
+    ws.hold()
+    ws.ensure(ws.nbytes + 1)
+    assert [b.data_ptr() for b in ws.held] == [held.data_ptr()] and ws.buf.data_ptr() != held.data_ptr()
+    ws.captured = True
+    with pytest.raises(ValueError, match="cannot grow"):
+        ws.ensure(ws.nbytes + 1)

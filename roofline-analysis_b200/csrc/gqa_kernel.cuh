@@ -45,6 +45,10 @@ namespace b2d {
 
 enum KvKind : int { kKvBf16 = 0, kKvFp16 = 1, kKvFp8 = 2 };
 
+// The running maximum before any score: finite, so that a score of -inf is no
+// NaN against it but a weight of 0.
+constexpr float kNoMax = -3.4028234663852886e38f;
+
 struct GqaParams {
   const void* q;
   int64_t q_sb, q_sh;
@@ -331,7 +335,7 @@ __global__ void __maxnreg__(B2D_GQA_MAXNREG)
 
   float2 q[HQW][4];
   float2 acc[HQW][4];
-  float m_own = -INFINITY, l_own = 0.f;   // online-softmax state of the own head
+  float m_own = kNoMax, l_own = 0.f;      // online-softmax state of the own head
   int cur_row = -1;
   int L = 0;
   float vscale = 1.f;
@@ -352,7 +356,7 @@ __global__ void __maxnreg__(B2D_GQA_MAXNREG)
       }
     }
     const float lse2_own = m_own + fast_log2(l_own);
-    const float inv_own = 1.f / l_own;
+    const float inv_own = l_own == 0.f ? 0.f : 1.f / l_own;   // no mass: out 0, lse -inf
     const int b = row / p.HG, hg = row - b * p.HG;
     const int cf = cta_of_chunk(row_start[row], W, G);
     const int cl = cta_of_chunk(row_start[row + 1] - 1, W, G);
@@ -412,7 +416,7 @@ __global__ void __maxnreg__(B2D_GQA_MAXNREG)
         acc[h][e] = make_float2(0.f, 0.f);
       }
     }
-    m_own = -INFINITY;
+    m_own = kNoMax;
     l_own = 0.f;
   };
 
@@ -594,9 +598,10 @@ __device__ __forceinline__ void warp_merge_heads(const GqaParams& p, int b, int 
 #pragma unroll
       for (int e = 0; e < EPL; ++e) acc[e] *= r;
       mx = bm;
+      const float mz = fmaxf(mx, kNoMax);   // (every part so far without mass: weights 0)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float w = (j0 + u < nseg) ? fast_exp2(lv[u] - mx) : 0.f;
+        const float w = (j0 + u < nseg) ? fast_exp2(lv[u] - mz) : 0.f;
         wsum += w;
 #pragma unroll
         for (int e = 0; e < EPL / 2; ++e) {
@@ -608,7 +613,7 @@ __device__ __forceinline__ void warp_merge_heads(const GqaParams& p, int b, int 
     if (live) {
       const int qh = hg * HQC + qh_row;
       const int64_t at = (int64_t)b * p.o_sb + (int64_t)qh * p.o_sh + hl * EPL;
-      const float inv = 1.f / wsum;
+      const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
       if constexpr (F32) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) p.out_f32[at + e] = acc[e] * inv;
@@ -705,6 +710,7 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(const GqaParams p, int
     for (int j = lane; j < nseg; j += 32) mx = fmaxf(mx, p.part_lse[(seg0 + j) * HQC + qh_row]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = fmaxf(mx, kNoMax);   // (every part without mass: weights 0)
     for (int j0 = sub * U; j0 < nseg; j0 += wpp * U) {
       float lv[U];
       float2 v[U][EPL / 2];
@@ -742,7 +748,7 @@ __global__ void __launch_bounds__(256) gqa_combine_kernel(const GqaParams p, int
     }
   }
   if (mode == 2 && sub == 0) {
-    const float inv = 1.f / wsum;
+    const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) put(e, acc[e] * inv);
     if (p.lse != nullptr && lane == 0) p.lse[(int64_t)b * p.lse_sb + qh] = (mx + fast_log2(wsum)) * kLn2;

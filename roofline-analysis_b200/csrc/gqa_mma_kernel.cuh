@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
-    m_r[0] = m_r[1] = -INFINITY;
+    m_r[0] = m_r[1] = kNoMax;
     l_r[0] = l_r[1] = 0.f;
   };
 
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
         const float lh = __shfl_sync(0xffffffffu, l_r[n], src);
         const float mh = __shfl_sync(0xffffffffu, m_r[n], src);
         if (hw >= GW) continue;
-        const float inv = vscale / lh;
+        const float inv = lh == 0.f ? 0.f : vscale / lh;   // no mass: out 0, lse -inf
         const int qh_row = qh_row0 + hw;
         if (cf == cl) {
           const int64_t at = (int64_t)b * p.o_sb + (int64_t)(hg * HQC + qh_row) * p.o_sh;
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const float mn = fmaxf(m_r[r], rmax[r]);
-        alpha[r] = (mn == -INFINITY) ? 1.f : fast_exp2(m_r[r] - mn);
+        alpha[r] = fast_exp2(m_r[r] - mn);
         m_r[r] = mn;
         l_r[r] *= alpha[r];
       }

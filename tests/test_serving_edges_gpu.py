@@ -297,3 +297,52 @@ def test_buffer_of_a_captured_decode_outlives_growth(cuda):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
     assert all((f == 77).all() for f in fill)
     b200decode.check_device_status(ws)
+
+
+# ---------------------------------------------------------------- rows without mass
+
+def minus_infinity(k, P, layout, row, n):
+    """Makes every score of a row's first n tokens -inf for positive queries."""
+    for pos in range(n):
+        pg, off = int(row[pos // P]), pos % P
+        if layout == "vllm":
+            k[pg, :, 0, off, 0] = float("-inf")
+        elif layout == "HND":
+            k[pg, :, off, 0] = float("-inf")
+        else:
+            k[pg, off, :, 0] = float("-inf")
+
+
+@pytest.mark.parametrize("num_ctas", [None, 1, 40])
+@pytest.mark.parametrize("qd,hq,hkv,d,P,layout", [
+    (BF, 8, 2, 128, 16, "NHD"), (HF, 4, 4, 64, 16, "HND"), (BF, 32, 2, 128, 16, "NHD"), (BF, 8, 2, 128, 5, "NHD"),
+    (BF, 8, 2, 256, 16, "NHD"), (BF, 4, 2, 128, 16, "vllm")])
+def test_shared_prefix_of_own_tokens_without_mass(cuda, qd, hq, hkv, d, P, layout, num_ctas):
+    """Own tokens whose scores are all -inf (the first of them, all, all of a
+    long sequence) weigh nothing beside the prefix; with no prefix: 0 and -inf."""
+    plens, lens, starts = [150, 0], [40, 700, 3, 33, 40], [0, 3, 5]
+    gen, k, v, ks, vs, both = paged(cuda, 320, plens + lens, P, hkv, d, qd, layout)
+    pbt, bt = both[:2], both[2:]
+    gone = [40, 700, 1, 20, 40]
+    for b, n in enumerate(gone):
+        minus_infinity(k, P, layout, bt[b], n)
+    q = torch.rand(5, hq, d, generator=gen, device=cuda).add_(0.1).to(qd)
+    kw = dict(kv_layout=layout, num_ctas=num_ctas)
+    out, lse = b200decode.decode_shared_prefix(q, k, v, i32(plens), pbt, i32(lens), bt, group_starts=i32(starts), **kw)
+    alone, alone_lse = b200decode.decode(q, k, v, i32(lens), bt, **kw)
+    one, one_lse = b200decode.cross_attention(q, k, v, i32(lens), bt, **kw)
+    torch.cuda.synchronize()
+    b200decode.check_device_status()
+    for b, n in enumerate(lens):
+        kk, vv = gather(k, ks, bt[b], n, lay(layout, "k"))[gone[b]:], gather(v, vs, bt[b], n, lay(layout, "v"))[gone[b]:]
+        own = attend(q[b:b + 1].double(), kk, vv, d ** -0.5, qd)
+        r = own
+        if b < 3:
+            pre = attend(q[b:b + 1].double(), gather(k, ks, pbt[0], 150, lay(layout, "k")),
+                         gather(v, vs, pbt[0], 150, lay(layout, "v")), d ** -0.5, qd)
+            r = merge2(own, pre)
+        check(out[b:b + 1], r[0], r[2], u_of(qd), "out")
+        check_lse(lse[b:b + 1], r[1], r[3])
+        for o, l in ((alone, alone_lse), (one, one_lse)):
+            check(o[b:b + 1], own[0], own[2], u_of(qd), "own tokens alone")
+            check_lse(l[b:b + 1], own[1], own[3])

@@ -294,9 +294,9 @@ __device__ __forceinline__ void load_lane(const float* src, float* v) {
 // sum) in their join, and the join's log2 sum.  A part without mass gets 0.
 __device__ __forceinline__ float2 join_weights(float a2, float own, float& lse2) {
   const float b2 = own * 1.4426950408889634f, mx = fmaxf(a2, b2);
-  if (mx == -INFINITY) {
-    lse2 = a2 + b2;   // -inf, or NaN
-    return make_float2(1.f, 0.f);
+  if (mx == -INFINITY) {   // no mass, or NaN beside none (fmaxf leaves a NaN out)
+    lse2 = a2 + b2;
+    return make_float2(lse2 == -INFINITY ? 1.f : lse2, 0.f);
   }
   const float wa = fast_exp2(a2 - mx), wb = fast_exp2(b2 - mx), inv = 1.f / (wa + wb);
   lse2 = mx + fast_log2(wa + wb);

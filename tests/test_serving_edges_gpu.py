@@ -346,3 +346,21 @@ def test_shared_prefix_of_own_tokens_without_mass(cuda, qd, hq, hkv, d, P, layou
         for o, l in ((alone, alone_lse), (one, one_lse)):
             check(o[b:b + 1], own[0], own[2], u_of(qd), "own tokens alone")
             check_lse(l[b:b + 1], own[1], own[3])
+
+
+@pytest.mark.parametrize("num_ctas", [None, 1, 7])
+@pytest.mark.parametrize("P", [16, 5])
+def test_shared_prefix_without_mass_keeps_a_nan_of_the_own_tokens(cuda, P, num_ctas):
+    """A NaN among a sequence's own keys makes its rows NaN, also beside a
+    prefix whose scores are all -inf; its neighbours are right."""
+    gen, k, v, _, _, both = paged(cuda, 330, [200, 30, 30, 30], P, 2, 64, BF)
+    pbt, bt = both[:1], both[1:]
+    minus_infinity(k, P, "NHD", pbt[0], 200)
+    k[bt[1, 17 // P].long(), 17 % P, :, 3] = float("nan")
+    q = torch.rand(3, 4, 64, generator=gen, device=cuda).add_(0.1).to(BF)
+    out, lse = b200decode.decode_shared_prefix(q, k, v, i32([200]), pbt, i32([30] * 3), bt, num_ctas=num_ctas)
+    assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
+    for b in (0, 2):
+        r = attend(q[b:b + 1].double(), gather(k, None, bt[b], 30, "NHD"), gather(v, None, bt[b], 30, "NHD"), 0.125, BF)
+        check(out[b:b + 1], r[0], r[2] * (1 + 2.0 ** -11), u_of(BF), "out")
+        check_lse(lse[b:b + 1], r[1], r[3] + 2.0 ** -20 * (1 + r[1].abs()))

@@ -135,7 +135,8 @@ __device__ __forceinline__ float q_at(const QT* qrow, bool valid, int dim) {
 // ([head][D][16 tokens], 32-byte rows, no swizzle) and feed the P.V product
 // through plain (non-transposing) ldmatrix.
 // F32: out goes to p.out_f32 (a kernel of its own: the choice at run time cost
-// the FP8 decode 0.8 %).
+// the FP8 decode 0.8 %), and weights in fp16 are 2^15 as large as they are, so
+// that those far below the largest keep their bits (ragged_tc_kernel.cuh).
 template <int D, int KIND, typename QT, int NP, bool VL = false, bool F32 = false>
 __global__ void __launch_bounds__(32 * 9, 1)
     gqa_mma_kernel(const __grid_constant__ CUtensorMap tmap_k,
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
   constexpr int MT = D / 16;                     // PV m-tiles (dims)
   constexpr int T = 16;                          // tokens per chunk
   constexpr float kLn2 = 0.69314718055994530942f;
+  constexpr float kUp = F32 && !MMA_BF16 ? 15.f : 0.f;
 
   extern __shared__ __align__(1024) uint8_t smem[];
   const int R = p.B * p.HG;
@@ -337,6 +339,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
         const float mh = __shfl_sync(0xffffffffu, m_r[n], src);
         if (hw >= GW) continue;
         const float inv = lh == 0.f ? 0.f : vscale / lh;   // no mass: out 0, lse -inf
+        const float lse2 = mh + (fast_log2(lh) - kUp);
         const int qh_row = qh_row0 + hw;
         if (cf == cl) {
           const int64_t at = (int64_t)b * p.o_sb + (int64_t)(hg * HQC + qh_row) * p.o_sh;
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
             }
           }
           if (p.lse != nullptr && g == 0)
-            p.lse[(int64_t)b * p.lse_sb + hg * HQC + qh_row] = (mh + fast_log2(lh)) * kLn2;
+            p.lse[(int64_t)b * p.lse_sb + hg * HQC + qh_row] = lse2 * kLn2;
         } else {
           const int64_t seg = (int64_t)row + cta;
           float* dst = p.part_o + (seg * HQC + qh_row) * D;
@@ -365,7 +368,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
             dst[out_dim(i, 0)] = acc[n][i][c] * inv;
             dst[out_dim(i, 1)] = acc[n][i][2 + c] * inv;
           }
-          if (g == 0) p.part_lse[seg * HQC + qh_row] = mh + fast_log2(lh);
+          if (g == 0) p.part_lse[seg * HQC + qh_row] = lse2;
         }
       }
     }
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(32 * 9, 1)
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float pv = fast_exp2(sfr[j][e] - m_r[e >> 1]);
+        const float pv = fast_exp2(sfr[j][e] - (m_r[e >> 1] - kUp));
         sfr[j][e] = pv;
         l_r[e >> 1] += pv;
       }

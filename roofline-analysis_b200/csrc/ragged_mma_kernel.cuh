@@ -10,7 +10,8 @@
 // layout of the second).  K and V come in with plain 16-byte loads through
 // the block table, one token at a time, so a page may end anywhere; e4m3 is
 // converted to fp16 (exact) on the way.  Keys past the end are zero-filled
-// and masked.  Rows in shared memory are padded by 16 bytes, so the 8 row
+// and masked.  Weights in fp16 are 2^15 as large as they are, so that small ones
+// keep their bits (ragged_tc_kernel.cuh).  Rows in shared memory are padded by 16 bytes, so the 8 row
 // addresses of an ldmatrix fall into different banks.
 #pragma once
 
@@ -50,7 +51,7 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
   using C = RaggedMma<D>;
   constexpr bool BF = KIND == kKvBf16;             // e4m3 and fp16 caches: fp16 products
   constexpr int CH = C::kCH, LD = C::kLd, NT = CH / 8, KS = D / 16;
-  constexpr float kLn2 = 0.69314718055994530942f;
+  constexpr float kLn2 = 0.69314718055994530942f, kUp = BF ? 0.f : 15.f;
   extern __shared__ __align__(16) uint8_t smem[];
   uint16_t* sq = reinterpret_cast<uint16_t*>(smem);
   uint16_t* sk = sq + C::kRows * LD;
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[j][e] = fast_exp2(s[j][e] - mz[e >> 1]);
+          s[j][e] = fast_exp2(s[j][e] - (mz[e >> 1] - kUp));
           l[e >> 1] += s[j][e];
         }
 #pragma unroll
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
       const int row = 16 * warp + gq + 8 * r;
       if (row >= nrows) continue;
       float inv = l[r] > 0.f ? vscale / l[r] : l[r];   // no mass at all: 0; NaN stays
-      float lse2 = m[r] + fast_log2(l[r]);
+      float lse2 = m[r] + (fast_log2(l[r]) - kUp);
       const int t = t0 + row / p.grp, h = w.h * p.grp + row % p.grp;
       if (whole) {
         if (p.own_o != nullptr) {   // join with the sequence's own part

@@ -25,7 +25,10 @@
 // The maximum is lazy: it moves only when a score exceeds it by 2^8, so P <=
 // 256 and O is rescaled (a TMEM round trip) rarely: a chunk that leaves it, or
 // sets it first, goes from S to P in registers, any other takes the general
-// step.
+// step.  In fp16, whose smallest number is 2^-24, P is 2^7 as large (at most
+// 2^15): of a long sequence beside a dominant key, the many weights far below
+// it keep their bits (20000 of 2^-24.3 each were 27 % off, of 2^-26 all lost).
+// The sum is of the same scaled weights, so only lse has to take the 7 back.
 //
 // Keys past the end: their pages are not loaded, their scores are masked, and
 // warp 11 (e4m3: the conversion) zeroes their V rows, which may hold anything,
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   constexpr bool BF = KIND == kKvBf16;
   constexpr bool F8 = C::kFp8;
   constexpr int CH = C::kCH, NS = C::kSlots, NR = C::kRawSlots;
-  constexpr float kLazy = 8.f;
+  constexpr float kLazy = 8.f, kUp = BF ? 0.f : 7.f;
   constexpr float kLn2 = 0.69314718055994530942f;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           float vscale = 1.f;
           if constexpr (F8) vscale = p.v_scale ? __ldg(p.v_scale + d.head(st)) : 1.f;
           float inv = l > 0.f ? vscale / l : l;
-          float lse2 = l == 0.f ? -INFINITY : m * sl + fast_log2(l);
+          float lse2 = l == 0.f ? -INFINITY : m * sl + (fast_log2(l) - kUp);
           const int tok = d.t0 + d.first(st, p.TS) + tq, head = d.head(st) * p.grp + hq;
           const bool join = whole && p.own_o != nullptr;
           float own = 0.f;                         // weight of the sequence's own part
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
           }
         }
         // A score of NaN or +inf makes the whole row NaN, by way of l.
-        const float off = !(cm < INFINITY) ? NAN : m == -INFINITY ? 0.f : -m * sl;
+        const float off = !(cm < INFINITY) ? NAN : m == -INFINITY ? 0.f : fmaf(-m, sl, kUp);
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
         for (int c = 0; c < CH; c += 32) {
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
         // (a NaN, an infinite maximum, or +inf against a finite one fail this)
         if (!__all_sync(0xffffffffu, (cm - mn) * sl <= kLazy && fabsf(mn) < INFINITY)) return false;
         m = mn;
-        const float off = -m * sl;
+        const float off = fmaf(-m, sl, kUp);
         float2 s0 = make_float2(0.f, 0.f), s1 = s0;
 #pragma unroll
         for (int c = 0; c < CH; c += 32) {

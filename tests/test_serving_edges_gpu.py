@@ -364,3 +364,51 @@ def test_shared_prefix_without_mass_keeps_a_nan_of_the_own_tokens(cuda, P, num_c
         r = attend(q[b:b + 1].double(), gather(k, None, bt[b], 30, "NHD"), gather(v, None, bt[b], 30, "NHD"), 0.125, BF)
         check(out[b:b + 1], r[0], r[2] * (1 + 2.0 ** -11), u_of(BF), "out")
         check_lse(lse[b:b + 1], r[1], r[3] + 2.0 ** -20 * (1 + r[1].abs()))
+
+
+# ---------------------------------------------------------------- small weights
+
+@pytest.mark.parametrize("num_ctas", [None, 1])
+@pytest.mark.parametrize("score", [16.875, 18.0])
+@pytest.mark.parametrize("kv,d,P", [(HF, 64, 16), (F8, 128, 16), (HF, 128, 5), (HF, 256, 16), (F8, 64, 5)])
+def test_many_weights_far_below_the_largest(cuda, kv, d, P, score, num_ctas):
+    """One key holds nearly all the weight and a value of 0, as an attention
+    sink does; thousands of equal weights of e^-score beside it make the whole
+    output.  In fp16 as they are, they would be multiples of 2^-24 of a value
+    near one of them (or 0); the kernels scale them by 2^7 or more first, so each
+    is off by at most 2^-32 of the largest."""
+    n = 20000
+    gen, k, v, _, _, bt = paged(cuda, 340, [n, n, 16], P, 1, d, kv)
+    scale = 1.0 if score == 18.0 else 0.9375                  # (both exact, in e4m3 too)
+    k.copy_(torch.zeros(k.shape, device=cuda).to(kv))
+    v.copy_(torch.ones(v.shape, device=cuda).to(kv))
+    sink, zero = torch.zeros(1, d, device=cuda), torch.zeros(1, d, device=cuda)
+    sink[0, 0] = 18.0
+    for b, pos in ((0, 0), (1, n - 3), (2, 1)):
+        pg, off = bt[b, pos // P].long(), pos % P
+        k[pg, off] = sink.to(kv)
+        v[pg, off] = zero.to(kv)
+    q = torch.zeros(9, 2, d, device=cuda, dtype=HF)
+    q[:, :, 0] = 1
+
+    def near(out, lse, r):
+        u = 2.0 ** -11
+        # scores are exact; sums of n terms, powers and the join in fp32: n 2^-24 + 2^-17
+        tol = r[0].abs() * (u + n * 2.0 ** -24 + 2.0 ** -17) + n * 2.0 ** -32
+        check(out, r[0], tol, u_of(HF), "out")
+        check_lse(lse, r[1], r[3])
+
+    ref = [attend(q[:1].double(), gather(k, None, bt[b], m, "NHD"), gather(v, None, bt[b], m, "NHD"), scale, kv)
+           for b, m in ((0, n), (1, n), (2, 16))]
+    out, lse = b200decode.cross_attention(q, k, v, i32([n, n, 16]), bt, scale, query_starts=i32([0, 4, 6, 9]),
+                                          num_ctas=num_ctas)
+    for b, (lo, hi) in enumerate(((0, 4), (4, 6), (6, 9))):
+        for t in range(lo, hi):
+            near(out[t:t + 1], lse[t:t + 1], ref[b])
+    # the long tail in the prefix, and in the own tokens
+    both = merge2(ref[0], ref[2])
+    for pl, ol, pb, ob in ((n, 16, bt[:1], bt[2:]), (16, n, bt[2:], bt[:1])):
+        out, lse = b200decode.decode_shared_prefix(q, k, v, i32([pl]), pb, i32([ol] * 9), ob.repeat(9, 1), scale,
+                                                   num_ctas=num_ctas)
+        for t in range(9):
+            near(out[t:t + 1], lse[t:t + 1], both)

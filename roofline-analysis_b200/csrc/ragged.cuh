@@ -114,22 +114,30 @@ __host__ __device__ constexpr size_t ragged_table_bytes(int groups) {
   return ((size_t)groups + 1 + 32 + (groups <= kCachedGroups ? 3 * (size_t)groups : 0)) * 4;
 }
 
-// Fills the table (block-wide scan; ends with __syncthreads).  False, with a
-// table of no work: the starts descend somewhere.  Tokens would then belong to
-// several groups, whose rows race, and the work line could pass 32 bits (the
-// host's bound counts every token once).
-__device__ __forceinline__ bool ragged_table(const RaggedParams& p, int32_t* table) {
+// Set when the starts descend somewhere.  Tokens would then belong to several
+// groups, whose rows race, and the work line could pass 32 bits (the host's
+// bound counts every token once): the table is one of no work, and no row is
+// written.  It lies in the last int of the scratch, of which a block's warps use
+// at most 16.  (As a variable that lives across the kernel it cost 2 % on long
+// calls: 838 -> 857 us for 16 requests of up to 1024 x 6500 tokens.)
+__device__ __forceinline__ int32_t& ragged_descends(const RaggedParams& p, int32_t* table) {
+  return table[p.G + 32];
+}
+
+// Fills the table (block-wide scan; ends with __syncthreads).
+__device__ __forceinline__ void ragged_table(const RaggedParams& p, int32_t* table) {
   int32_t* warp_tmp = table + p.G + 1;
   int32_t* cache = p.G <= kCachedGroups ? warp_tmp + 32 : nullptr;
   const int tid = threadIdx.x, nth = blockDim.x;
   const int lane = tid & 31, warp = tid >> 5, nwarps = nth >> 5;
+  if (tid == 0) ragged_descends(p, table) = 0;
+  __syncthreads();
   int carry = 0;
-  bool descends = false;
   for (int base = 0; base < p.G; base += nth) {
     const int g = base + tid;
     int n = 0;
     if (g < p.G) {
-      descends = descends || (p.starts != nullptr && __ldg(p.starts + g + 1) < __ldg(p.starts + g));
+      if (p.starts != nullptr && __ldg(p.starts + g + 1) < __ldg(p.starts + g)) ragged_descends(p, table) = 1;
       const int2 tok = ragged_tokens(p, g);
       const int len = ragged_kv_len(p, g), nch = (len + p.CH - 1) / p.CH;
       n = nch > 0 ? ragged_items(p, tok.y) * (nch + kItemCost) : 0;
@@ -162,11 +170,12 @@ __device__ __forceinline__ bool ragged_table(const RaggedParams& p, int32_t* tab
     __syncthreads();
     carry += total;
   }
-  descends = __syncthreads_or(descends);
-  if (tid == 0) table[p.G] = descends ? 0 : carry;
-  if (descends && tid == 0 && blockIdx.x == 0) record_status(p.status, kStatusBounds);
+  if (tid == 0) {
+    const bool descends = ragged_descends(p, table) != 0;
+    table[p.G] = descends ? 0 : carry;
+    if (descends && blockIdx.x == 0) record_status(p.status, kStatusBounds);
+  }
   __syncthreads();
-  return !descends;
 }
 
 // A piece of an item, inside one range: chunks [c0, c1) of nch.  Part s (0 or
@@ -326,7 +335,8 @@ __device__ __forceinline__ void ragged_row_without_keys(const RaggedParams& p, i
 // All rows of groups without keys, and (shared prefix) of tokens outside every
 // group, spread over the blocks and their warps.
 template <int D, typename QT>
-__device__ __forceinline__ void ragged_rows_without_keys(const RaggedParams& p) {
+__device__ __forceinline__ void ragged_rows_without_keys(const RaggedParams& p, int32_t* table) {
+  if (ragged_descends(p, table) != 0) return;
   const int warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
   auto rows = [&](int t0, int n, int first, int step) {
     for (int64_t i = first; i < (int64_t)n * p.Hq; i += step)

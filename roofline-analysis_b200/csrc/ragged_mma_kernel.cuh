@@ -62,7 +62,8 @@ __global__ void __launch_bounds__(128) ragged_mma_kernel(const RaggedParams p) {
 
   griddep_wait();
   griddep_launch();
-  if (ragged_table(p, table)) ragged_rows_without_keys<D, QT>(p);
+  ragged_table(p, table);
+  ragged_rows_without_keys<D, QT>(p, table);
   const int W = table[p.G];
   const int ctas = W < (int)gridDim.x ? W : (int)gridDim.x;
   if (tid == 0) ragged_note_cut(p, blockIdx.x, nullptr, W, ctas);   // nothing yet

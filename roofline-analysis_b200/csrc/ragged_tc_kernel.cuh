@@ -197,10 +197,10 @@ __global__ void __launch_bounds__(RaggedTc<D, KIND>::kThreads, 1)
   // are read (and before the block ends, for the merge).
   if (!p.beside) griddep_wait();
   griddep_launch();
-  const bool sane = ragged_table(p, table);  // ends with __syncthreads
+  ragged_table(p, table);                    // ends with __syncthreads
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (sane) ragged_rows_without_keys<D, QT>(p);
+  ragged_rows_without_keys<D, QT>(p, table);
   const int W = table[p.G];
   const int ctas = W < (int)gridDim.x ? W : (int)gridDim.x;
   const bool active = (int)blockIdx.x < ctas;

@@ -576,7 +576,7 @@ __device__ __forceinline__ void warp_merge_heads(const GqaParams& p, int b, int 
     float acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
-    float wsum = 0.f, mx = -INFINITY;
+    float wsum = 0.f, mx = kNoMax;
     for (int j0 = 0; j0 < nseg; j0 += U) {
       float lv[U];
       float2 v[U][EPL / 2];
@@ -593,15 +593,14 @@ __device__ __forceinline__ void warp_merge_heads(const GqaParams& p, int b, int 
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (j0 + u < nseg) bm = fmaxf(bm, lv[u]);
-      const float r = (mx == -INFINITY) ? 0.f : fast_exp2(mx - bm);
+      const float r = fast_exp2(mx - bm);
       wsum *= r;
 #pragma unroll
       for (int e = 0; e < EPL; ++e) acc[e] *= r;
       mx = bm;
-      const float mz = fmaxf(mx, kNoMax);   // (every part so far without mass: weights 0)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float w = (j0 + u < nseg) ? fast_exp2(lv[u] - mz) : 0.f;
+        const float w = (j0 + u < nseg) ? fast_exp2(lv[u] - mx) : 0.f;
         wsum += w;
 #pragma unroll
         for (int e = 0; e < EPL / 2; ++e) {

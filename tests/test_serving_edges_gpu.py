@@ -412,3 +412,91 @@ def test_many_weights_far_below_the_largest(cuda, kv, d, P, score, num_ctas):
                                                    num_ctas=num_ctas)
         for t in range(9):
             near(out[t:t + 1], lse[t:t + 1], both)
+
+
+# ---------------------------------------------------------------- errors that a bound for each element does not see
+
+def spread(got, q, k, v, scale, kv, qd):
+    """Mean of (error / s)^2 over all elements, s^2 = (u_out out)^2 + u_p^2 sum_j (p_j v_j)^2.
+    The rounding of out is off by at most u_out |out|, and each weight, rounded
+    to 16 bits by itself, by at most u_p of its size, with no common sign: were
+    all at their limits the mean would be 1, as they are spread it is about 1/3.
+    (fp32 errors of scores and sums are under 2^-18 of a weight.)  A part that is
+    lost, misplaced or misweighted shows long before it passes the bound for
+    each element, which adds up all weights' errors."""
+    T, hq, d = q.shape
+    grp = hq // k.shape[1]
+    k, v = k.repeat_interleave(grp, 1), v.repeat_interleave(grp, 1)
+    p = torch.softmax(torch.einsum("thd,lhd->thl", q.double(), k) * scale, -1)
+    out = torch.einsum("thl,lhd->thd", p, v)
+    u_p = 2.0 ** -8 if kv == BF else 2.0 ** -11
+    s2 = (u_of(qd) * out) ** 2 + u_p ** 2 * torch.einsum("thl,lhd->thd", p ** 2, v ** 2)
+    return float((((got.double() - out) ** 2) / s2).mean())
+
+
+@pytest.mark.parametrize("num_ctas", [None, 5])
+@pytest.mark.parametrize("qd,kv,hq,hkv,d,P", [(BF, BF, 8, 2, 128, 16), (HF, HF, 4, 4, 64, 64), (BF, F8, 16, 2, 128, 16),
+                                              (BF, BF, 8, 2, 128, 5), (HF, HF, 4, 1, 256, 16)])
+def test_spread_of_errors(cuda, qd, kv, hq, hkv, d, P, num_ctas):
+    lens, tq = [9000, 1000, 130], [40, 140, 9]
+    gen, k, v, ks, vs, bt = paged(cuda, 370, lens, P, hkv, d, kv)
+    q = torch.randn(189, hq, d, generator=gen, device=cuda).to(qd)
+    out, _ = b200decode.cross_attention(q, k, v, i32(lens), bt, query_starts=i32([0, 40, 180, 189]), k_scale=ks,
+                                        v_scale=vs, num_ctas=num_ctas)
+    for b, (lo, hi) in enumerate(((0, 40), (40, 180), (180, 189))):
+        kk, vv = gather(k, ks, bt[b], lens[b], "NHD"), gather(v, vs, bt[b], lens[b], "NHD")
+        assert spread(out[lo:hi], q[lo:hi], kk, vv, d ** -0.5, kv, qd) < 1
+    # own tokens behind a prefix: request 0's keys, then request 1's or 2's
+    own = [1 + i % 2 for i in range(20)]
+    out, _ = b200decode.decode_shared_prefix(q[:20], k, v, i32(lens[:1]), bt[:1], i32([lens[b] for b in own]),
+                                             bt[torch.tensor(own)], k_scale=ks, v_scale=vs, num_ctas=num_ctas)
+    for b in (1, 2):
+        kk, vv = (torch.cat([gather(c, s, bt[x], lens[x], "NHD") for x in (0, b)]) for c, s in ((k, ks), (v, vs)))
+        assert spread(out[b - 1:20:2], q[b - 1:20:2], kk, vv, d ** -0.5, kv, qd) < 1
+
+
+@pytest.mark.parametrize("num_ctas", [None, 3, 29])
+@pytest.mark.parametrize("kv,d,P", [(BF, 128, 16), (HF, 64, 48), (F8, 128, 16), (BF, 128, 5), (BF, 192, 16)])
+def test_every_border_token_counts_once(cuda, kv, d, P, num_ctas):
+    """V is 1 in a dim of its own for a few tokens, at the borders of pages,
+    chunks and sequences, and 0 elsewhere: that dim of out is the token's own
+    weight, off by its two roundings and no more."""
+    n = 3000
+    lens = [n, 130]
+    gen, k, v, ks, _, bt = paged(cuda, 380, lens, P, 2, d, kv)
+    at = sorted({x for c in (0, P, 128, 256, 1024, 1536, 2048, n - 1, n - P) for x in (c - 1, c, c + 1) if 0 <= x < n})
+    at += [x for x in range(700, n, 131) if x not in at][:d - len(at)]
+    v.copy_(torch.zeros(v.shape, device=cuda).to(kv))
+    for i, pos in enumerate(at):
+        row = torch.zeros(2, d, device=cuda)
+        row[:, i] = 1
+        v[bt[0, pos // P].long(), pos % P] = row.to(kv)
+        if pos < 130:
+            v[bt[1, pos // P].long(), pos % P] = row.to(kv)
+    q = (0.3 * torch.randn(70, 8, d, generator=gen, device=cuda)).to(HF if kv == HF else BF)
+
+    def weights(qq, keys, parts, got):
+        s = torch.einsum("thd,lhd->thl", qq.double(), keys.repeat_interleave(4, 1)) * d ** -0.5
+        p, want = torch.softmax(s, -1), torch.zeros(qq.shape, dtype=torch.float64, device=cuda)
+        for base, length in parts:
+            for i, pos in enumerate(at):
+                if pos < length:
+                    want[..., i] += p[..., base + pos]
+        # a weight rounded to 16 bits (fp16: scaled, so 2^-32 of the largest at least); its score and the
+        # maximum off by ds each (serving_ref.py); powers, sums and the join in fp32; out rounded by check()
+        u_p, least = (2.0 ** -8, 0.0) if kv == BF else (2.0 ** -11, 2.0 ** -32)
+        s_abs = torch.einsum("thd,lhd->thl", qq.double().abs(), keys.abs().repeat_interleave(4, 1)).amax(-1) * d ** -0.5
+        ds = 2.0 ** -24 * (d + 4) * s_abs[..., None]
+        check(got, want, want * (u_p + 2 * ds + keys.shape[0] * 2.0 ** -24 + 2.0 ** -17) + least, u_of(got.dtype), "weights")
+
+    ks = ks if kv == F8 else None
+    k0, k1 = (gather(k, ks, bt[b], m, "NHD") for b, m in ((0, n), (1, 130)))
+    out, _ = b200decode.cross_attention(q, k, v, i32(lens), bt, query_starts=i32([0, 60, 70]), k_scale=ks,
+                                        num_ctas=num_ctas)
+    weights(q[:60], k0, [(0, n)], out[:60])
+    weights(q[60:], k1, [(0, 130)], out[60:])
+    for pre, own in ((0, 1), (1, 0)):
+        out, _ = b200decode.decode_shared_prefix(q[:33], k, v, i32([lens[pre]]), bt[pre:pre + 1], i32([lens[own]] * 33),
+                                                 bt[own:own + 1].repeat(33, 1), k_scale=ks, num_ctas=num_ctas)
+        both = torch.cat([(k0, k1)[pre], (k0, k1)[own]])
+        weights(q[:33], both, [(0, lens[pre]), (lens[pre], lens[own])], out)

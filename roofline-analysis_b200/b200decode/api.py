@@ -63,6 +63,7 @@ class DecodeWorkspace:
         self.lock = threading.RLock()
         self.captured = False   # a CUDA graph holds this buffer's address: it may not grow
         self.held: list = []    # buffers that graphs of decode() calls hold, kept as long as the workspace
+        self.graph_made = False  # allocated under capture: zeroed by the graph's replay, not before
         self.buf = self._alloc(max(nbytes, 1 << 20))
 
     @classmethod
@@ -71,7 +72,7 @@ class DecodeWorkspace:
         graph's pool, its header zeroed by a node of the graph."""
         ws = cls.__new__(cls)
         ws.device, ws.stream, ws.captured = torch.device(device), None, True
-        ws.lock, ws.held = threading.RLock(), []
+        ws.lock, ws.held, ws.graph_made = threading.RLock(), [], True
         ws.buf = torch.empty(max(nbytes, _lib.B2D_WORKSPACE_HEADER_BYTES), dtype=torch.uint8, device=device)
         ws.buf[:_lib.B2D_WORKSPACE_HEADER_BYTES].zero_()
         return ws
@@ -87,16 +88,35 @@ class DecodeWorkspace:
 
     def _alloc(self, n: int) -> torch.Tensor:
         with self._on_stream():
+            self.graph_made = self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
             return torch.zeros(n, dtype=torch.uint8, device=self.device)
+
+    def eager(self) -> "DecodeWorkspace":
+        """For a call outside of capture: a buffer that a capture allocated is
+        left to the graph (its header is not zero yet), and another one taken."""
+        if self.graph_made:
+            with self.lock:
+                if self.graph_made:
+                    self.hold()
+                    self.buf = self._alloc(self.buf.numel())
+        return self
+
+    def for_decode(self, nbytes: int) -> None:
+        """The buffer of a decode(): under capture it is held for the graph."""
+        if torch.cuda.is_current_stream_capturing():
+            self.ensure(nbytes).hold()
+        else:
+            self.eager().ensure(nbytes)
 
     def ensure(self, nbytes: int) -> "DecodeWorkspace":
         if self.buf.numel() < nbytes:
             if self.captured:
                 raise ValueError(f"a workspace that a CUDA graph holds cannot grow (it has {self.buf.numel()} "
                                  f"bytes, {nbytes} are needed): size it before the capture")
-            old, self.buf = self.buf, self._alloc(int(nbytes * 1.25) + 4096)
+            old, unset = self.buf, self.graph_made
+            self.buf = self._alloc(int(nbytes * 1.25) + 4096)
             # a status that was recorded and not read stays (a graph under capture would copy it at each replay)
-            if not (old.is_cuda and torch.cuda.is_current_stream_capturing()):
+            if not unset and not self.graph_made:
                 with self._on_stream():
                     self.buf[:_STATUS_BYTES].copy_(old[:_STATUS_BYTES])
         return self
@@ -259,9 +279,7 @@ def decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     _check(lib.b2d_gqa_workspace_bytes(C.byref(a), C.byref(need)), "b2d_gqa_workspace_bytes")
     stream = torch.cuda.current_stream(q.device).cuda_stream
     with ws.lock:
-        ws.ensure(need.value)
-        if torch.cuda.is_current_stream_capturing():
-            ws.hold()
+        ws.for_decode(need.value)
         a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
         _check(lib.b2d_decode_gqa(C.byref(a), C.c_void_p(stream)), "b2d_decode_gqa")
     return out, lse
@@ -302,7 +320,7 @@ class GqaDecoder:
         _check(self._lib.b2d_gqa_workspace_bytes(C.byref(self._args), C.byref(need)),
                "b2d_gqa_workspace_bytes")
         with self.ws.lock:
-            self.ws.ensure(need.value)
+            self.ws.for_decode(need.value)
             self._ws_buf = self.ws.buf   # pin the buffer this plan points at
             self._args.workspace, self._args.workspace_bytes = self.ws.ptr, self.ws.nbytes
         self._argp = C.byref(self._args)
@@ -397,9 +415,7 @@ def decode_mla(q: torch.Tensor, kv_cache: torch.Tensor, cache_seqlens: torch.Ten
     _check(lib.b2d_mla_workspace_bytes(C.byref(a), C.byref(need)), "b2d_mla_workspace_bytes")
     stream = torch.cuda.current_stream(q.device).cuda_stream
     with ws.lock:
-        ws.ensure(need.value)
-        if torch.cuda.is_current_stream_capturing():
-            ws.hold()
+        ws.for_decode(need.value)
         a.workspace, a.workspace_bytes = ws.ptr, ws.nbytes
         _check(lib.b2d_decode_mla(C.byref(a), C.c_void_p(stream)), "b2d_decode_mla")
     return out, lse

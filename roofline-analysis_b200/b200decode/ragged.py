@@ -74,10 +74,10 @@ def _workspace(workspace: Optional[DecodeWorkspace], index: int, need: Callable[
         if workspace.buf.get_device() != index:
             raise ValueError(f"workspace is on {workspace.buf.device}, the tensors on cuda:{index}")
         workspace.captured = workspace.captured or capturing
-        return workspace.ensure(need()) if capturing else workspace
+        return workspace.ensure(need()) if capturing else workspace.eager()
     if capturing:
         return DecodeWorkspace.in_graph(torch.device("cuda", index), need())
-    return _ws.get((index, _stream(index))) or _default_ws(torch.device("cuda", index))
+    return (_ws.get((index, _stream(index))) or _default_ws(torch.device("cuda", index))).eager()
 
 
 def _call(fn, name: str, a, own, workspace: Optional[DecodeWorkspace], index: int, query) -> None:

@@ -500,3 +500,29 @@ def test_every_border_token_counts_once(cuda, kv, d, P, num_ctas):
                                                  bt[own:own + 1].repeat(33, 1), k_scale=ks, num_ctas=num_ctas)
         both = torch.cat([(k0, k1)[pre], (k0, k1)[own]])
         weights(q[:33], both, [(0, lens[pre]), (lens[pre], lens[own])], out)
+
+
+def test_first_capture_of_a_stream_leaves_eager_calls_a_zeroed_workspace(cuda):
+    """A decode() captured on a stream that has no workspace yet; then, before
+    any replay, steps on that stream whose blocks count themselves in the header."""
+    gen, k, v, _, _, bt = paged(cuda, 390, [500, 300], 16, 2, 128, BF)
+    q, kl = torch.randn(2, 8, 128, generator=gen, device=cuda).to(BF), i32([500, 300])
+    want = b200decode.decode(q, k, v, kl, bt)
+    b200decode.cross_attention(q, k, v, kl, bt, query_starts=i32([0, 1, 2]))
+    B, P = 4000, 16
+    lens, table = torch.zeros(B, dtype=torch.int32, device=cuda), torch.zeros(B, 2, dtype=torch.int32, device=cuda)
+    free, count = torch.arange(B, dtype=torch.int32, device=cuda), i32([B])
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        got = b200decode.decode(q, k, v, kl, bt)
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            b200decode.plan_append(lens, table, free, count, P, seqlens_out=lens, free_count_out=count)
+        s.synchronize()
+        b200decode.check_device_status()
+        assert (lens == 3).all() and int(count) == 0
+        g.replay()
+        s.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

@@ -84,3 +84,24 @@ def test_held_buffer_outlives_growth(host):
     ws.captured = True
     with pytest.raises(ValueError, match="cannot grow"):
         ws.ensure(ws.nbytes + 1)
+
+
+def test_buffer_made_under_capture_is_left_to_the_graph(host, monkeypatch):
+    """A buffer that a capture allocated is zeroed by the graph's replay, not
+    before: calls outside of the capture take another one."""
+    ws = DecodeWorkspace(host)
+    first = ws.buf
+    ws.graph_made = True                       # (as _alloc() notes on a GPU)
+    ws.buf.fill_(0xAB)                         # what such memory may hold
+    ws.for_decode(1000)
+    assert ws.buf.data_ptr() != first.data_ptr() and not ws.buf.any() and not ws.graph_made
+    assert [b.data_ptr() for b in ws.held] == [first.data_ptr()]
+    ws.graph_made = True
+    ws.buf.fill_(0xAB)
+    a = _lib.GqaArgs()
+    entry = Entry(ws, {0: 1})
+    ragged._call(entry, "entry", a, a, ws, -1, entry.query)
+    assert not ws.buf.any() and len(ws.held) == 2 and all(at_buf for _, _, at_buf in entry.log)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    ws.for_decode(1000)
+    assert ws.held[-1] is ws.buf

@@ -258,9 +258,14 @@ int b2d_append_kv(const b2d_append_args* args, void* stream);
  *   lse        [num_tokens, num_q_heads] fp32 (may be NULL)
  * A request without states yields out = 0 and lse = -inf; tokens behind
  * query_starts[num_groups] are left as they were.  Starts that descend: out and
- * lse are left as they were and the status word reports B2D_ERR_DEVICE_BOUNDS.
+ * lse are left as they were (of the 4096 requests around the place: longer lists
+ * run in slices) and the status word reports B2D_ERR_DEVICE_BOUNDS.
  * out overlaps no input.
  * head_dim 64, 128, 192 and 256, group (num_q_heads / num_kv_heads) <= 32.
+ * Precision: the softmax weights enter the second product rounded to 16 bits
+ * (the caches' type; fp16 for e4m3 caches), sums and the softmax are fp32.  With
+ * e4m3 caches the queries enter the first product in fp16: bf16 values beyond
+ * 65504 become infinite (their rows NaN), those under 2^-14 lose bits.
  */
 typedef struct b2d_cross_args {
   const void* q;
@@ -313,7 +318,8 @@ int b2d_cross_attention(const b2d_cross_args* args, void* stream);
  *              that descend: as those of b2d_cross_args.
  * Either part may be empty; both: out = 0, lse = -inf.  out overlaps no input.
  * num_groups <= 4096.  Sizes as b2d_decode_gqa takes them: it runs the own
- * tokens, and B2D_ERR_UNSUPPORTED for own is the answer here too.
+ * tokens, and B2D_ERR_UNSUPPORTED for own is the answer here too.  Precision as
+ * b2d_cross_attention; both parts are joined in fp32 and rounded once.
  */
 typedef struct b2d_shared_prefix_args {
   b2d_gqa_args own;

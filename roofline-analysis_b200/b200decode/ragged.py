@@ -159,6 +159,11 @@ def cross_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     query_starts that descend are reported (check_device_status(),
     B2D_ERR_DEVICE_BOUNDS) and nothing is written.
 
+    Softmax and sums are fp32; the softmax weights enter the second product
+    rounded to 16 bits (the caches' type, fp16 for e4m3).  With e4m3 caches q
+    enters the first product in fp16: bf16 values beyond 65504 become infinite
+    (their rows NaN), those under 2^-14 lose bits.
+
     Captured into a CUDA graph without `workspace`, a call keeps its scratch
     in the graph's memory pool; check_device_status() reads the status only of
     a workspace that the caller passes.
@@ -269,9 +274,9 @@ def decode_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     hold here too: the query heads of a KV head split into at most 8 equal
     parts of at most 16 (8 at head_dim 192 and 256); with pages that are no
     multiples of 16, or e4m3 at head_dim 64, they are at most 8, or 16 if even;
-    head_dim 192 takes 16-bit caches in pages of multiples of 16 alone.
-    Out is computed in fp32 over both parts and rounded once;
-    it must not overlap q.
+    head_dim 192 takes 16-bit caches in pages of multiples of 16 alone.  The
+    two parts, each as precise as cross_attention()'s, are joined in fp32 and
+    rounded once; out must not overlap q.
 
     With a table whose rows begin with a common prefix of n full pages, pass
     prefix_block_table = table[:1, :n], block_table = table[:, n:] and the

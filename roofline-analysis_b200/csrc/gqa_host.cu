@@ -243,12 +243,16 @@ static int launch_k(Kern kern, void (*combine)(const GqaParams, int, int), const
   // rows (small batches, rows over ~100 CTAs) the multi-warp combine kernel
   // spreads the merges instead.  B2D_GQA_FUSED_MERGE=0/1 forces either.
   static const int fused_env = env_int("B2D_GQA_FUSED_MERGE", -1);
-  // The fp32 output of a shared-prefix call is merged in the kernel whenever no
-  // row has more than kMaxPieces pieces, because the prefix kernel, which starts
-  // while this one runs, hides the merge but waits for a combine launch.  Whole
-  // call, 1024 shared keys, 32 on 8 heads, combine / in the kernel: 4 sequences
-  // with 256 own keys 31.4 / 26.1 us, 2048 (37 pieces) 32.8 / 37.2; 32 with 600
-  // 44.4 / 37.8; 256 with 600 135.6 / 132.0.
+  // The fp32 output of a shared-prefix call is merged in the kernel where rows
+  // have up to kMaxPieces pieces (by the width of the block table, none can have
+  // more), or have on average, because the prefix kernel, which starts while this
+  // one runs, hides the merge but waits for a combine launch.  The lengths are on
+  // the device, so one long row among short ones is merged by one warp all the
+  // same.  Whole call, 1024 shared keys, 32 on 8 heads, combine / in the kernel: 4
+  // sequences with 256 own keys 31.4 / 26.1 us, 2048 (37 pieces) 32.8 / 37.2; 8
+  // with 600 33.5 / 46.4; 16 with 600 36.9 / 32.8, with 8000 104.1 / 98.6; 32 with
+  // 600 44.4 / 37.8; 256 with 600 135.6 / 132.0; 16, one with 30000 and 15 with 50:
+  // 54 / 101.
   constexpr int kMaxPieces = 24;
   const int64_t row_chunks = ((int64_t)p.max_pages * p.P + p.T - 1) / p.T;
   const bool in_kernel = (int64_t)R * 7 >= ctas ||

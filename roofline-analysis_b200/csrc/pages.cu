@@ -16,6 +16,11 @@
 // place: then the block that is last to finish reading (an arrival counter in
 // the workspace header, zero between calls) writes them.  A thread takes 4
 // slots at a time, so that their table reads are in flight together.
+//
+// A negative page never enters the pool: the blocks of a release copy the pages
+// above the top of the stack, where nothing counts yet, and tell the last one
+// whether they met a negative entry; it moves the top, or leaves everything.
+// (The wait for the last block: 512 requests, a tenth finished, 6.5 -> 7.1 us.)
 #include "b2d_decode.h"
 #include "common.cuh"
 #include "host_common.h"

@@ -156,6 +156,10 @@ static int make_plan(const b2d_gqa_args* a, GqaPlan* pl) {
     if (cap_hk < 1) cap_hk = 1;
     pl->hk = largest_divisor_leq(a->num_kv_heads, cap_hk);
     pl->T = 16;
+    // Two stages of K and V have to fit an SM (8 heads of 256 would not).
+    constexpr int kTwoStages = 200 * 1024;
+    while (pl->hk > 1 && 4 * pl->T * pl->hk * a->head_dim * es > kTwoStages)
+      pl->hk = largest_divisor_leq(a->num_kv_heads, pl->hk / 2);
     // Small problems (few sequences, short caches): narrower tiles give more
     // chunks, so every CTA still gets about two.  The chunk count is bounded
     // by the block table's width; the lengths themselves live on the device.

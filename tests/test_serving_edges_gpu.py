@@ -526,3 +526,25 @@ def test_first_capture_of_a_stream_leaves_eager_calls_a_zeroed_workspace(cuda):
         g.replay()
         s.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("hkv,grp,d", [(8, 1, 256), (16, 4, 256), (7, 2, 256), (8, 4, 192)])
+def test_wide_rows_of_many_heads(cuda, hkv, grp, d):
+    """Eight KV heads of 256 dims do not fit a tile: narrower ones are taken
+    (with a table wide enough that the batch alone would ask for wide tiles)."""
+    lens, plen = [700, 1, 0, 333] * 16, 60
+    gen, k, v, _, _, both = paged(cuda, 295, lens + [plen], 16, hkv, d, BF)
+    bt, pbt = both[:64], both[64:, :4]
+    q = torch.randn(64, hkv * grp, d, generator=gen, device=cuda).to(BF)
+    wide = torch.zeros(64, 600, dtype=torch.int32, device=cuda)
+    wide[:, :bt.shape[1]] = bt
+    got = [b200decode.decode(q, k, v, i32(lens), wide), b200decode.cross_attention(q, k, v, i32(lens), wide),
+           b200decode.decode_shared_prefix(q, k, v, i32([plen]), pbt, i32(lens), wide)]
+    torch.cuda.synchronize()
+    b200decode.check_device_status()
+    for b in (0, 1, 2, 3, 40, 63):
+        part = [attend(q[b:b + 1].double(), gather(k, None, r, m, "NHD"), gather(v, None, r, m, "NHD"), d ** -0.5, BF)
+                for r, m in ((bt[b], lens[b]), (pbt[0], plen))]
+        for (out, lse), ref in zip(got, (part[0], part[0], merge2(*part))):
+            check(out[b:b + 1], ref[0], ref[2], u_of(BF), "out")
+            check_lse(lse[b:b + 1], ref[1], ref[3])

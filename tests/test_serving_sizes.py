@@ -41,3 +41,22 @@ def test_cross_takes_every_group_and_shared_prefix_what_decode_takes(d, page, kv
         assert refused == [g for g in range(1, 33) if not any(g % w == 0 and g // w <= most for w in range(1, 9))]
     else:
         assert refused == [g for g in range(1, 33) if g > (8 if g % 2 else 16)]
+
+
+@pytest.mark.parametrize("kv_heads", [1, 4, 6, 7, 8, 16])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("kv", [BF, F8])
+def test_two_stages_of_a_tile_fit_an_sm(kv_heads, d, kv):
+    """K and V tiles of 16 tokens, two stages of each, in 227 KB of shared memory,
+    for tables of any width (short ones have narrower tiles)."""
+    if kv == F8 and d == 192:
+        return
+    lib, a = _lib.load(), _lib.GqaArgs()
+    ctas, tokens, heads = C.c_int32(), C.c_int32(), C.c_int32()
+    for columns in (1, 100, 1 << 16):
+        sizes(a, 4, d, 16, kv)
+        a.batch, a.num_kv_heads, a.num_q_heads, a.max_pages_per_seq = 64, kv_heads, 4 * kv_heads, columns
+        assert lib.b2d_gqa_plan(C.byref(a), C.byref(ctas), C.byref(tokens), C.byref(heads)) == 0
+        assert kv_heads % heads.value == 0
+        # beside the tiles: barriers, up to 2049 row starts, scan and alignment
+        assert 4 * tokens.value * heads.value * d * (1 if kv == F8 else 2) <= 227 * 1024 - 10 * 1024

@@ -299,13 +299,13 @@ def decode_shared_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
         _ints(where, "group_starts", group_starts, groups + 1)
     elif groups > 1:
         raise ValueError(f"{where}: {groups} prefixes need group_starts")
+    if q.dim() == 4 and q.shape[1] != 1:
+        raise ValueError(f"{where}: one query token per sequence (q [B, 1, Hq, D]), got {tuple(q.shape)}")
     q3 = q[:, 0] if q.dim() == 4 else q
     if q3.dim() != 3:
         raise ValueError(f"{where}: q must be [B, Hq, D] or [B, 1, Hq, D], got {tuple(q.shape)}")
     shape = q3.shape
     _ints(where, "cache_seqlens", cache_seqlens, shape[0])
-    if q.dim() == 4 and q.shape[1] != 1:
-        raise ValueError(f"{where}: one query token per sequence (q [B, 1, Hq, D]), got {tuple(q.shape)}")
     if softmax_scale is None:
         softmax_scale = shape[-1] ** -0.5
     if out is None:

@@ -548,3 +548,13 @@ def test_wide_rows_of_many_heads(cuda, hkv, grp, d):
         for (out, lse), ref in zip(got, (part[0], part[0], merge2(*part))):
             check(out[b:b + 1], ref[0], ref[2], u_of(BF), "out")
             check_lse(lse[b:b + 1], ref[1], ref[3])
+
+
+def test_shared_prefix_refuses_no_token(cuda):
+    """q [B, 0, Hq, D] and [B, 2, Hq, D]: a ValueError of the call's own."""
+    k = torch.zeros(4, 16, 2, 64, dtype=BF, device=cuda)
+    kl, bt = i32([16, 16]), i32([[0], [1]])
+    for n in (0, 2):
+        q = torch.zeros(2, n, 4, 64, dtype=BF, device=cuda)
+        with pytest.raises(ValueError, match="one query token"):
+            b200decode.decode_shared_prefix(q, k, k, kl[:1], bt[:1], kl, bt)

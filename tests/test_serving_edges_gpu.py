@@ -558,3 +558,115 @@ def test_shared_prefix_refuses_no_token(cuda):
         q = torch.zeros(2, n, 4, 64, dtype=BF, device=cuda)
         with pytest.raises(ValueError, match="one query token"):
             b200decode.decode_shared_prefix(q, k, k, kl[:1], bt[:1], kl, bt)
+
+
+# ---------------------------------------------------------------- every kernel
+
+def draw(rng, i, pages, dims):
+    """A random size, of the warp-level kernel where the pages or dims ask for it."""
+    kv = rng.choice([BF, HF, F8])
+    qd = HF if kv == HF else rng.choice([BF, HF]) if kv == F8 else BF
+    d, P, layout = rng.choice(dims), rng.choice(pages), rng.choice(["NHD", "HND", "vllm"])
+    if layout == "vllm" and (kv == F8 or P % 16):
+        layout = "NHD"
+    return kv, qd, rng.choice([1, 2, 3, 5, 8]), d, P, layout
+
+
+@pytest.mark.parametrize("part", range(4))
+def test_cross_fuzz_of_the_warp_level_kernel(cuda, part):
+    import random
+    rng = random.Random(100 + part)
+    for i in range(15):
+        kv, qd, hkv, d, P, layout = draw(rng, i, [1, 2, 5, 7, 8, 16, 24, 100, 128], [64, 128, 192, 256])
+        grp = rng.choice([1, 2, 3, 5, 7, 8, 13, 16, 29, 32])
+        lens = [rng.choice([0, 1, 31, 32, 33, 63, 64, 65, rng.randint(1, 700)]) for _ in range(rng.randint(1, 5))]
+        tq = [rng.choice([0, 1, 2, rng.randint(1, 90)]) for _ in lens]
+        starts = [sum(tq[:b]) for b in range(len(tq) + 1)]
+        if starts[-1] == 0:
+            continue
+        gen, k, v, ks, vs, bt = paged(cuda, 400 + 20 * part + i, lens, P, hkv, d, kv, layout)
+        q = torch.randn(starts[-1], hkv * grp, d, generator=gen, device=cuda).to(qd)
+        out, lse = b200decode.cross_attention(q, k, v, i32(lens), bt, query_starts=i32(starts), k_scale=ks, v_scale=vs,
+                                              kv_layout=layout, num_ctas=rng.choice([None, None, 1, 2, 13, 300]))
+        for b, n in enumerate(lens):
+            s = slice(starts[b], starts[b + 1])
+            if tq[b]:
+                r = attend(q[s].double(), gather(k, ks, bt[b], n, lay(layout, "k")),
+                           gather(v, vs, bt[b], n, lay(layout, "v")), d ** -0.5, kv)
+                check(out[s], r[0], r[2], u_of(qd), f"{i}: out")
+                check_lse(lse[s], r[1], r[3])
+    b200decode.check_device_status()
+
+
+@pytest.mark.parametrize("part", range(6))
+def test_shared_fuzz(cuda, part):
+    import random
+    rng = random.Random(200 + part)
+    for i in range(15):
+        kv, qd, hkv, d, P, layout = draw(rng, i, [16, 16, 32, 48, 64, 112, 256, 1, 5, 8, 24], [64, 128, 128, 256])
+        grp = rng.choice([1, 2, 3, 4, 5, 6, 7, 8])
+        B, G = rng.randint(1, 40), rng.choice([1, 1, 2, 5])
+        cuts = sorted(rng.randint(0, B) for _ in range(G + 1))
+        plens = [rng.choice([0, 1, 127, 128, 129, rng.randint(1, 900)]) for _ in range(G)]
+        lens = [rng.choice([0, 1, 15, 16, 17, rng.randint(1, 300)]) for _ in range(B)]
+        gen, k, v, ks, vs, both = paged(cuda, 600 + 20 * part + i, plens + lens, P, hkv, d, kv, layout)
+        pbt, bt = both[:G], both[G:]
+        q = torch.randn(B, hkv * grp, d, generator=gen, device=cuda).to(qd)
+        out, lse = b200decode.decode_shared_prefix(q, k, v, i32(plens), pbt, i32(lens), bt, group_starts=i32(cuts),
+                                                   k_scale=ks, v_scale=vs, kv_layout=layout,
+                                                   num_ctas=rng.choice([None, None, 1, 3, 50, 400]))
+        for b in range(B):
+            one = lambda row, n: attend(q[b:b + 1].double(), gather(k, ks, row, n, lay(layout, "k")),   # noqa: E731
+                                        gather(v, vs, row, n, lay(layout, "v")), d ** -0.5, kv)
+            r = one(bt[b], lens[b])
+            for g in range(G):
+                if cuts[g] <= b < cuts[g + 1]:
+                    r = merge2(r, one(pbt[g], plens[g]))
+            check(out[b:b + 1], r[0], r[2], u_of(qd), f"{i}: out {b}")
+            check_lse(lse[b:b + 1], r[1], r[3])
+    b200decode.check_device_status()
+
+
+@pytest.mark.parametrize("d,P,layout,kv", [(128, 5, "NHD", BF), (256, 16, "HND", HF), (64, 7, "NHD", F8), (128, 16, "vllm", BF)])
+@pytest.mark.parametrize("num_ctas", [None, 1, 9])
+def test_warp_level_kernel_with_odd_values(cuda, d, P, layout, kv, num_ctas):
+    """NaN and infinity in a valid key stay with their request and KV head;
+    a page out of range is read as page 0 and reported; scales of either sign."""
+    lens, tq = [300, 150, 200], [40, 9, 30]
+    gen, k, v, ks, vs, bt = paged(cuda, 395, lens, P, 2, d, kv, layout)
+    if kv == F8:
+        ks[1] = -ks[1]
+    qd = HF if kv == HF else BF
+    q = torch.rand(79, 8, d, generator=gen, device=cuda).add_(0.1).to(qd)
+    st, kl = i32([0, 40, 49, 79]), i32(lens)
+    ws = b200decode.DecodeWorkspace(cuda, 64 << 20)
+    call = lambda kk, tt, scale: b200decode.cross_attention(   # noqa: E731
+        q, kk, v, kl, tt, scale, query_starts=st, k_scale=ks, v_scale=vs, kv_layout=layout, num_ctas=num_ctas, workspace=ws)
+    for scale in (-0.05, 0.0, d ** -0.5):
+        out, lse = call(k, bt, scale)
+        for b, (lo, hi) in enumerate(((0, 40), (40, 49), (49, 79))):
+            r = attend(q[lo:hi].double(), gather(k, ks, bt[b], lens[b], lay(layout, "k")),
+                       gather(v, vs, bt[b], lens[b], lay(layout, "v")), scale, kv)
+            check(out[lo:hi], r[0], r[2], u_of(qd), "out")
+            check_lse(lse[lo:hi], r[1], r[3])
+    b200decode.check_device_status(ws)
+    for pos in (0, 77, 299):
+        for value in (float("nan"), float("inf")):
+            if kv == F8 and value == float("inf"):
+                continue
+            bad = k.clone()
+            raw = bad.view(torch.uint8) if kv == F8 else bad
+            pg, off = int(bt[0, pos // P]), pos % P
+            at = (pg, 1, 0, off, 5) if layout == "vllm" else (pg, 1, off, 5) if layout == "HND" else (pg, off, 1, 5)
+            raw[at] = 0x7F if kv == F8 else value
+            got, _ = call(bad, bt, d ** -0.5)
+            assert torch.isnan(got[:40, 4:]).all() and torch.equal(got[:40, :4], out[:40, :4])
+            assert torch.equal(got[40:], out[40:])
+    for page in (-1, k.shape[0], 2 ** 31 - 1):
+        wrong, zero = bt.clone(), bt.clone()
+        wrong[1, 2], zero[1, 2] = page, 0
+        got, _ = call(k, wrong, d ** -0.5)
+        with pytest.raises(b200decode.B2DError) as e:
+            b200decode.check_device_status(ws)
+        assert e.value.code == -7
+        assert torch.equal(got, call(k, zero, d ** -0.5)[0])
